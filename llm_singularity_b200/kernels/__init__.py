@@ -950,6 +950,128 @@ def paged_attention(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, s
                   _p(out), _i(last - first), _i(ctx.max_q_len), *tail, skip, on)
 
 
+# ------------------------------------------------------ a cache of keys and values in 4 bits
+def kv4_head_ok(hd: int, page_size: int) -> bool:
+    """Whether a 4-bit cache holds heads of ``hd`` in pages of ``page_size`` tokens."""
+    return hd % 32 == 0 and 32 <= hd <= 256 and page_size > 0 and page_size % 16 == 0
+
+
+def _check_kv4(what: str, cache, nkv: int, hd: int) -> None:
+    if not kv4_head_ok(hd, cache.page_size):
+        raise KernelError(f"{what}: a 4-bit cache holds heads of a multiple of 32 up to 256 in pages of a multiple of 16 "
+                          f"tokens, got {hd} and {cache.page_size}")
+    pages = _req(cache.pages, "pages", torch.uint8, 4)
+    if nkv <= 0 or pages.shape[1:] != (nkv, cache.page_size // 16, 18 * hd):
+        raise KernelError(f"{what}: pages are {tuple(pages.shape)}, expected [pages, {nkv}, {cache.page_size // 16}, {18 * hd}]")
+    if pages.data_ptr() % 16 or pages.shape[0] * nkv * (cache.page_size // 16) > 0x7fffffff:
+        raise KernelError(f"{what}: pages must start at a multiple of 16 bytes and hold fewer than 2^31 tiles")
+    _req(cache.block_table, "block_table", torch.int32, 2)
+
+
+def _same_device(what: str, *tensors) -> None:
+    """Refuses tensors of different devices, and a device that is not the current one (its streams take no launches)."""
+    index = tensors[0].get_device()
+    if any(t is not None and t.get_device() != index for t in tensors):
+        raise KernelError(f"{what}: the tensors are on different devices")
+    if index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the tensors are on cuda:{index}, which is not the current device")
+
+
+def rope_kv4_store(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, inv_freq: Optional[torch.Tensor],
+                   rotary_dim: int, q_out: torch.Tensor, store: bool = True) -> None:
+    """From the fused projection ``qkv`` [T, (nh + 2 * nkv) * hd] to rotated queries in ``q_out`` [T, nh * hd] and, if
+    ``store``, keys and values in their places of the 4-bit cache.  The first ``rotary_dim`` dims of a head turn in pairs
+    (i, i + rotary_dim / 2) by position * inv_freq[i], the angle in 64-bit (``rope_kv_store``: in 32-bit).  Keys are rounded
+    to the compute type and then, like values, to 4 bits: every 32 dims of a head share a scale s, amax / 7 in 32-bit rounded
+    to 5 significant bits, and hold round(x / s) (ties to even) from -7 to 7.  A group whose largest magnitude is below
+    2^-100 holds zeros; one with a number that is not finite reads back as NaN."""
+    T = _check_rope(qkv, nh, nkv, hd, ctx, inv_freq, rotary_dim)
+    _check_kv4("rope_kv4_store", cache, nkv, hd)
+    _req(q_out, "q_out", qkv.dtype, 2)
+    if nh <= 0 or q_out.shape != (T, nh * hd):
+        raise KernelError(f"rope_kv4_store: q_out is {tuple(q_out.shape)}, expected {(T, nh * hd)}")
+    _same_device("rope_kv4_store", qkv, q_out, cache.pages, cache.block_table, inv_freq if rotary_dim else None)
+    _call("kv4_store", "lsb_rope_kv4_store", _p(qkv), _i(_dt(qkv)), _i(T), _i(nh), _i(nkv), _i(hd), _p(ctx.positions),
+          _p(ctx.token_req), _p(ctx.table_rows), _p(cache.block_table), _i(cache.block_table.shape[1]),
+          _p(inv_freq if rotary_dim else None), _i(rotary_dim), _p(q_out), _p(cache.pages), _i(cache.page_size),
+          _i(cache.pages.shape[0]), _i(1 if store else 0), _stream(qkv))
+
+
+def read_kv4(cache, nkv: int, hd: int, token_rows: torch.Tensor, positions: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor) -> None:
+    """What a 4-bit cache holds: for each i the key and the value, [nkv, hd], of the token at ``positions[i]`` of the
+    request with block-table row ``token_rows[i]``.  Exact in both compute types.  A place whose page the request does not
+    hold gives zeros and is recorded."""
+    _check_kv4("read_kv4", cache, nkv, hd)
+    _req(token_rows, "token_rows", torch.int32, 1)
+    _req(positions, "positions", torch.int32, 1)
+    n = positions.shape[0]
+    _req(k_out, "k_out", dim=3)
+    _req(v_out, "v_out", k_out.dtype, 3)
+    if token_rows.shape[0] != n or k_out.shape != (n, nkv, hd) or v_out.shape != k_out.shape:
+        raise KernelError(f"read_kv4: one row and one [{nkv}, {hd}] key and value for each of the {n} positions")
+    _same_device("read_kv4", k_out, v_out, cache.pages, cache.block_table, token_rows, positions)
+    _call("kv4_store", "lsb_read_kv4", _p(cache.pages), _p(token_rows), _p(positions), _p(cache.block_table),
+          _i(cache.block_table.shape[1]), _i(cache.block_table.shape[0]), _p(k_out), _p(v_out), _i(_dt(k_out)), _i(n), _i(nkv),
+          _i(hd), _i(cache.page_size), _i(cache.pages.shape[0]), _stream(k_out))
+
+
+_kv4_rooms: Dict[tuple, tuple] = {}
+
+
+def _kv4_room(lib: str, hd: int, eights: int, device) -> tuple:
+    """(blocks that the SMs hold at once, the largest cluster) of a kernel."""
+    key = (lib, hd, eights)
+    if key not in _kv4_rooms:
+        got = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights)))
+        _kv4_rooms[key] = (max(1, got >> 8) * num_sms(device), max(1, got & 255))
+    return _kv4_rooms[key]
+
+
+def paged_attention_kv4(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, scale: float, window: int,
+                        out: torch.Tensor, first: int = 0) -> None:
+    """Causal attention of this step's queries over a 4-bit cache: query head h of the token at position p sees the keys of
+    kv head h // (nh / nkv) at positions j <= p with j > p - ``window`` (0: all) or j < ``first``.  ``qkv``: rows that begin
+    with the token's rotated queries, [T, nh * hd] or longer.  Scores, softmax and sums are 32-bit; with bfloat16 rows a
+    probability times its value's scale is rounded to bfloat16."""
+    _req(qkv, "qkv", dim=2)
+    _req(out, "out", qkv.dtype, 2)
+    T = qkv.shape[0]
+    if nkv <= 0 or nh <= 0 or nh % nkv:
+        raise KernelError(f"paged_attention_kv4: {nh} heads cannot share {nkv} kv heads")
+    if qkv.shape[1] < nh * hd or out.shape != (T, nh * hd) or ctx.n_tokens != T:
+        raise KernelError("paged_attention_kv4: qkv, out and the step disagree")
+    if ctx.n_requests > 65535 or nkv > 65535:
+        raise KernelError("paged_attention_kv4: at most 65535 requests and kv heads per step")
+    if window < 0 or first < 0:
+        raise KernelError("paged_attention_kv4: the window and the number of first tokens must not be negative (0: none)")
+    _check_kv4("paged_attention_kv4", cache, nkv, hd)
+    _same_device("paged_attention_kv4", qkv, out, cache.pages, cache.block_table)
+    if out.data_ptr() % 16:
+        raise KernelError("paged_attention_kv4: out must start at a multiple of 16 bytes")
+    bf16, group, R = _dt(qkv) == _BF16, nh // nkv, ctx.n_requests
+    lib = "attention_kv4" if bf16 else "attention_kv4_f32"
+    n_single, begin, end = _batch_shape(ctx)
+    fixed = getattr(ctx, "fixed_launch", False)
+    for mode, at, count, requests, most in ((1, 0, R, n_single, 1), (2, begin, end - begin, R - n_single, ctx.max_q_len)):
+        if not requests:
+            continue
+        rows = most * group
+        eights = 2 if bf16 and hd <= 128 and rows > 8 else 1
+        room, cap = _kv4_room(lib, hd, eights, qkv.device)
+        blocks = requests * nkv * -(-rows // (8 * eights))
+        splits = max(1, min(cap, int(0.8 * room / blocks + 0.5)))
+        if not fixed:                               # (a captured launch has to serve contexts of any length)
+            longest = ctx.max_kv_len if not window else min(ctx.max_kv_len, window + most + first)
+            splits = min(splits, -(-longest // 128))
+        off = 4 * at
+        _call(lib, "lsb_attention_kv4", _p(qkv), _i(qkv.shape[1]), _p(cache.pages), ctypes.c_void_p(ctx.q_start.data_ptr() + off),
+              ctypes.c_void_p(ctx.kv_len.data_ptr() + off), ctypes.c_void_p(ctx.table_rows.data_ptr() + off),
+              _p(cache.block_table), _i(cache.block_table.shape[1]), _p(out), _i(count), _ll(rows), _i(nh), _i(nkv), _i(hd),
+              _i(cache.page_size), _i(cache.pages.shape[0]), _f(scale), _i(window), _i(first), _i(mode), _i(eights), _i(splits),
+              _stream(out))
+
+
 # ----------------------------------------------- rows of a stream that is normed after the sum
 def cast_rows(x: torch.Tensor, out: torch.Tensor) -> None:
     """out = x (32-bit) rounded to out's dtype."""

@@ -36,6 +36,9 @@ SOURCES: Dict[str, object] = {          # library -> its source file (or files)
     "attention": "attention.cu",
     "attention_tc": "attention_tc.cu",
     "attention_tc5": "attention_tc5.cu",
+    "kv4_store": "kv4_store.cu",
+    "attention_kv4": "attention_kv4.cu",
+    "attention_kv4_f32": "attention_kv4_f32.cu",
     "gemm": "gemm.cu",
     "gemm_f32": "gemm_f32.cu",
     "gemm_tc": "gemm_tc.cu",
@@ -63,7 +66,8 @@ SOURCES: Dict[str, object] = {          # library -> its source file (or files)
     # host code only: pools, block tables, prefix tree; scheduler
     "host_runtime": ("host_memory.cpp", "host_scheduler.cpp", "host_step.cpp"),
 }
-HEADERS = ["common.cuh", "attention_tc_noalloc.h", "attention_dv.cuh", "attention_tc5.cuh", "stream_warm.cuh", "gate_act.cuh"]     # of the CUDA libraries
+HEADERS = ["common.cuh", "attention_tc_noalloc.h", "attention_dv.cuh", "attention_tc5.cuh", "stream_warm.cuh", "gate_act.cuh",
+           "kv4.cuh", "attention_kv4.cuh"]     # of the CUDA libraries
 HOST_HEADERS = ["host_memory.h"]                          # of the host runtime
 
 

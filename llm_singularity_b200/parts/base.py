@@ -135,6 +135,18 @@ class PagedKVSpec(CacheSpec):
 
 
 @dataclass
+class KV4CacheView:
+    """What an attention call sees of a cache of keys and values in 4 bits (``csrc/kv4.cuh`` has the layout): a kv
+    head's 16 tokens are one tile of 18 * head_dim bytes."""
+
+    pages: torch.Tensor            # uint8 [num_pages, kv_heads, page_size / 16, 18 * head_dim]
+    block_table: torch.Tensor      # int32 [slots, max_pages]; rows picked by ctx.table_rows
+    page_size: int
+    window: Optional[int]
+    group: int
+
+
+@dataclass
 class LatentCacheView:
     """What a latent-attention call sees of its cache: one row per token."""
 
