@@ -956,7 +956,8 @@ def kv4_head_ok(hd: int, page_size: int) -> bool:
     return hd % 32 == 0 and 32 <= hd <= 256 and page_size > 0 and page_size % 16 == 0
 
 
-def _check_kv4(what: str, cache, nkv: int, hd: int) -> None:
+def _check_kv4(what: str, cache, nkv: int, hd: int):
+    """Refuses what is no 4-bit cache of ``nkv`` heads of ``hd``; its pages and block table."""
     if not kv4_head_ok(hd, cache.page_size):
         raise KernelError(f"{what}: a 4-bit cache holds heads of a multiple of 32 up to 256 in pages of a multiple of 16 "
                           f"tokens, got {hd} and {cache.page_size}")
@@ -965,7 +966,7 @@ def _check_kv4(what: str, cache, nkv: int, hd: int) -> None:
         raise KernelError(f"{what}: pages are {tuple(pages.shape)}, expected [pages, {nkv}, {cache.page_size // 16}, {18 * hd}]")
     if pages.data_ptr() % 16 or pages.shape[0] * nkv * (cache.page_size // 16) > 0x7fffffff:
         raise KernelError(f"{what}: pages must start at a multiple of 16 bytes and hold fewer than 2^31 tiles")
-    _req(cache.block_table, "block_table", torch.int32, 2)
+    return pages, _req(cache.block_table, "block_table", torch.int32, 2)
 
 
 def _same_device(what: str, *tensors) -> None:
@@ -1016,16 +1017,69 @@ def read_kv4(cache, nkv: int, hd: int, token_rows: torch.Tensor, positions: torc
           _i(hd), _i(cache.page_size), _i(cache.pages.shape[0]), _stream(k_out))
 
 
-_kv4_rooms: Dict[tuple, tuple] = {}
+_kv4_rooms: Dict[tuple, int] = {}
 
 
-def _kv4_room(lib: str, hd: int, eights: int, device) -> tuple:
-    """(blocks that the SMs hold at once, the largest cluster) of a kernel."""
-    key = (lib, hd, eights)
+def _kv4_room(lib: str, hd: int, eights: int, device) -> int:
+    """Blocks of a kernel that the device holds at once."""
+    key = (lib, hd, eights, device)
     if key not in _kv4_rooms:
-        got = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights)))
-        _kv4_rooms[key] = (max(1, got >> 8) * num_sms(device), max(1, got & 255))
+        _kv4_rooms[key] = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights))) * num_sms(device)
     return _kv4_rooms[key]
+
+
+def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int, capacity: int, device) -> list:
+    """The launches of a step's attention over a 4-bit cache, worked out once per step and kind of layer: (mode, offset into the
+    per-request arrays, requests, rows of a request, eights of rows of a block, blocks of a cluster, blocks of a spread launch, floats of
+    its parts).
+
+    Single tokens either have a cluster of blocks to each row tile, or are spread: equal stretches of all chunks of 32 tokens
+    for as many blocks as fit, and a kernel that joins what was cut.  The first ends when the longest context has ended (and has rounds
+    where blocks are more than fit), the second costs about 24 chunks a block more (measured, heads of 64 and 128 in bfloat16: 64
+    requests of 1,000 - 8,100 tokens 147 us with clusters of one, 107 spread; 64 of 4,096 55 and 59; 8 of 4,096 18 and 23;
+    one of 131,072 107 and 50).  A captured launch does not know the lengths: it is spread if the block tables have room for
+    long contexts."""
+    key = (lib, nh, nkv, hd, window, first, capacity)
+    plans = ctx.__dict__.setdefault("_kv4_plans", {})
+    if key in plans:
+        return plans[key]
+    n_single, begin, end = _batch_shape(ctx)
+    group, R, fixed = nh // nkv, ctx.n_requests, getattr(ctx, "fixed_launch", False)
+    plan = []
+    for mode, at, count, requests, most in ((1, 0, R, n_single, 1), (2, begin, end - begin, R - n_single, ctx.max_q_len)):
+        if not requests:
+            continue
+        rows = most * group
+        eights = 2 if lib == "attention_kv4" and hd <= 128 and rows > 8 else 1
+        tiles = requests * nkv * -(-rows // (8 * eights))
+        room = _kv4_room(lib, hd, eights, device)
+        seen = capacity if fixed else ctx.max_kv_len
+        if window:
+            seen = min(seen, window + most + first)
+        chunks = -(-seen // 32)                     # the most of a row tile
+        splits = spread = parts = 0
+        cost = None
+        for s in range(1, 9):
+            rounds = -(-tiles * s // room)
+            if s > 1 and (rounds > 1 or 4 * (s - 1) >= chunks):
+                break
+            c = rounds * -(-chunks // s) + (2 if s > 1 else 0)
+            if cost is None or c < cost:
+                splits, cost = s, c
+        if mode == 1 and R <= 256:
+            if fixed:
+                even = 0 if capacity >= 4096 else cost
+            else:
+                kv = ctx.h_kv_len if n_single == R else ctx.h_kv_len[ctx.h_q_len == 1]
+                if window:
+                    kv = kv.clip(max=window + first)
+                even = int(kv.sum()) * (tiles // requests) // (32 * room) + 24
+            if even < cost:
+                spread = max(room, tiles // requests)
+                parts = 2 * spread * int(_lib(lib).lsb_attention_kv4_slot(_i(hd), _i(eights)))
+        plan.append((mode, 4 * at, count, rows, eights, splits, spread, parts))
+    plans[key] = plan
+    return plan
 
 
 def paged_attention_kv4(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, scale: float, window: int,
@@ -1036,40 +1090,28 @@ def paged_attention_kv4(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cach
     probability times its value's scale is rounded to bfloat16."""
     _req(qkv, "qkv", dim=2)
     _req(out, "out", qkv.dtype, 2)
-    T = qkv.shape[0]
+    T, ld = qkv.shape
     if nkv <= 0 or nh <= 0 or nh % nkv:
         raise KernelError(f"paged_attention_kv4: {nh} heads cannot share {nkv} kv heads")
-    if qkv.shape[1] < nh * hd or out.shape != (T, nh * hd) or ctx.n_tokens != T:
+    if ld < nh * hd or out.shape != (T, nh * hd) or ctx.n_tokens != T:
         raise KernelError("paged_attention_kv4: qkv, out and the step disagree")
     if ctx.n_requests > 65535 or nkv > 65535:
         raise KernelError("paged_attention_kv4: at most 65535 requests and kv heads per step")
     if window < 0 or first < 0:
         raise KernelError("paged_attention_kv4: the window and the number of first tokens must not be negative (0: none)")
-    _check_kv4("paged_attention_kv4", cache, nkv, hd)
-    _same_device("paged_attention_kv4", qkv, out, cache.pages, cache.block_table)
+    pages, table = _check_kv4("paged_attention_kv4", cache, nkv, hd)
+    _same_device("paged_attention_kv4", qkv, out, pages, table)
     if out.data_ptr() % 16:
         raise KernelError("paged_attention_kv4: out must start at a multiple of 16 bytes")
-    bf16, group, R = _dt(qkv) == _BF16, nh // nkv, ctx.n_requests
-    lib = "attention_kv4" if bf16 else "attention_kv4_f32"
-    n_single, begin, end = _batch_shape(ctx)
-    fixed = getattr(ctx, "fixed_launch", False)
-    for mode, at, count, requests, most in ((1, 0, R, n_single, 1), (2, begin, end - begin, R - n_single, ctx.max_q_len)):
-        if not requests:
-            continue
-        rows = most * group
-        eights = 2 if bf16 and hd <= 128 and rows > 8 else 1
-        room, cap = _kv4_room(lib, hd, eights, qkv.device)
-        blocks = requests * nkv * -(-rows // (8 * eights))
-        splits = max(1, min(cap, int(0.8 * room / blocks + 0.5)))
-        if not fixed:                               # (a captured launch has to serve contexts of any length)
-            longest = ctx.max_kv_len if not window else min(ctx.max_kv_len, window + most + first)
-            splits = min(splits, -(-longest // 128))
-        off = 4 * at
-        _call(lib, "lsb_attention_kv4", _p(qkv), _i(qkv.shape[1]), _p(cache.pages), ctypes.c_void_p(ctx.q_start.data_ptr() + off),
-              ctypes.c_void_p(ctx.kv_len.data_ptr() + off), ctypes.c_void_p(ctx.table_rows.data_ptr() + off),
-              _p(cache.block_table), _i(cache.block_table.shape[1]), _p(out), _i(count), _ll(rows), _i(nh), _i(nkv), _i(hd),
-              _i(cache.page_size), _i(cache.pages.shape[0]), _f(scale), _i(window), _i(first), _i(mode), _i(eights), _i(splits),
-              _stream(out))
+    lib = "attention_kv4" if _dt(qkv) == _BF16 else "attention_kv4_f32"
+    window, first, width = min(window, 1 << 30), min(first, 1 << 30), table.shape[1]
+    q_start, kv_len, rows_of = ctx.q_start.data_ptr(), ctx.kv_len.data_ptr(), ctx.table_rows.data_ptr()
+    for mode, off, count, rows, eights, splits, spread, parts in _kv4_plan(ctx, lib, nh, nkv, hd, window, first,
+                                                                           width * cache.page_size, qkv.device):
+        scratch = torch.empty(parts, dtype=torch.float32, device=qkv.device) if spread else None
+        _call(lib, "lsb_attention_kv4", _p(qkv), ld, _p(pages), ctypes.c_void_p(q_start + off), ctypes.c_void_p(kv_len + off),
+              ctypes.c_void_p(rows_of + off), _p(table), width, _p(out), count, _ll(rows), nh, nkv, hd, cache.page_size,
+              pages.shape[0], _f(scale), window, first, mode, eights, splits, spread, _p(scratch), _stream(out))
 
 
 # ----------------------------------------------- rows of a stream that is normed after the sum

@@ -72,12 +72,12 @@ def step(q_lens, kv_lens, rows=None, fixed=False):
         q_start=dev(start), kv_len=dev(kv), table_rows=dev(rows), fixed_launch=fixed)
 
 
-def attention(q, K, V, L, scale, window, first):
-    """64-bit attention of q [n, heads, hd] (the last n of L positions) over K, V [L, kv heads, hd]: the result, the sum of
-    weights times the values' magnitudes, and the greatest size that a row's scores could have had without cancellation."""
+def attention(q, K, V, L, scale, window, first, steps):
+    """64-bit attention of q [n, heads, hd] (the last n of L positions) over K, V [L, kv heads, hd]: the result, and the sums of
+    weights times the values' magnitudes and times their ``steps`` [L, kv heads, hd] (the scale of each value's group)."""
     n, nh, hd = q.shape
     group = nh // K.shape[1]
-    K, V = (x.double().repeat_interleave(group, 1) for x in (K, V))
+    K, V, steps = (x.double().repeat_interleave(group, 1) for x in (K, V, steps))
     s = torch.einsum("ihd,jhd->hij", q.double(), K) * scale
     pos, key = torch.arange(L - n, L, device=q.device)[:, None], torch.arange(L, device=q.device)
     hidden = key > pos
@@ -87,4 +87,4 @@ def attention(q, K, V, L, scale, window, first):
     live = torch.where(hidden, torch.zeros_like(w), w)
     V0, hide = torch.nan_to_num(V, nan=0.0), hidden.all(0)
     V0 = torch.where(hide[:, None, None], torch.zeros_like(V0), V0)
-    return torch.einsum("hij,jhd->ihd", live, V0), torch.einsum("hij,jhd->ihd", live, V0.abs())
+    return tuple(torch.einsum("hij,jhd->ihd", live, x) for x in (V0, V0.abs(), torch.nan_to_num(steps, nan=0.0)))

@@ -144,7 +144,7 @@ def _case(ops, dtype, nh, nkv, hd, q_lens, kv_lens, window=0, first=0, page_size
     pages, table = _pool(R, max(kv_lens), nkv, hd, page_size, seed)
     scale = 1.0 / math.sqrt(hd) if scale is None else scale
     q = (torch.randn(T, nh * hd + extra, device="cuda", generator=g) * 1.5).to(dtype)
-    K, V = [], []
+    K, V, steps = [], [], []
     host = pages.cpu()
     for r, L in enumerate(kv_lens):
         k, v = (torch.randn(L, nkv, hd, device="cuda", generator=g) * torch.exp(spread * torch.randn(hd, device="cuda", generator=g))
@@ -155,6 +155,7 @@ def _case(ops, dtype, nh, nkv, hd, q_lens, kv_lens, window=0, first=0, page_size
         (kc, ks), (vc, vs) = rounded(k), rounded(v)
         K.append(values_of(kc, ks))
         V.append(values_of(vc, vs))
+        steps.append(vs.repeat_interleave(32, -1))
         lo = max(0, L - q_lens[r] - window + 1) if window else 0
         kr, vr = row_bytes(kc, False).cpu(), row_bytes(vc, True).cpu()
         G = hd // 32
@@ -179,19 +180,22 @@ def _case(ops, dtype, nh, nkv, hd, q_lens, kv_lens, window=0, first=0, page_size
         got = out[t:t + n].view(n, nh, hd).double()
         blind = torch.isnan(K[r]).any(-1).any(-1) | torch.isnan(V[r]).any(-1).any(-1)
         k0 = torch.where(blind[:, None, None], torch.zeros_like(K[r]), K[r])
-        want, size = attention(qr, k0, torch.where(blind[:, None, None], torch.full_like(V[r], math.nan), V[r]), L, scale, window, first)
+        v0 = torch.where(blind[:, None, None], torch.full_like(V[r], math.nan), V[r])
+        want, size, per_step = attention(qr, k0, v0, L, scale, window, first, steps[r])
         pos, key = torch.arange(L - n, L, device="cuda")[:, None], torch.arange(L, device="cuda")
         sees = (key <= pos) & ((key > pos - window) | (key < first)) if window else key <= pos
         spoilt = (sees & blind).any(-1)
         assert bool(torch.isnan(got[spoilt]).all()), r
-        # Scores: within a group of 32 dims an accumulator holds at most 279 |q|_1 (136 times the sum of q, and codes up to 143) with
-        # bfloat16 rows, and 36 additions each lose at most 2^-24 of that; with 32-bit rows 7 |q|_1 and three times the additions.  An
-        # exponential of 2^-22, the sum over L weights and the merges are within 2^-18 of a weight.  With bfloat16 rows a weight
-        # times its scale is rounded (half a step: 2^-8), and so is the result.
+        # Scores: within a group of 32 dims an accumulator holds at most 1,039 |q|_1 (a code's 1,024 + 15, and 1,032 taken off) with
+        # bfloat16 rows, and 36 additions each lose at most 2^-24 of that; with 32-bit rows 7 |q|_1 and three times the additions.
+        # An exponential of 2^-22, the sum over L weights and the merges are within 2^-18 of a weight.  With bfloat16 rows a
+        # weight times its scale is rounded (half a step: 2^-8), codes of up to 143 of it are summed over 32 tokens and 136 times
+        # their weights taken off again (36 additions), and the result is rounded.
         reach = (qr.double().abs().unflatten(-1, (-1, 32)).sum(-1).amax(0).amax(0) * torch.nan_to_num(k0).abs().unflatten(-1, (-1, 32)).amax(-1).amax(0).amax(0) / 7).sum().item()
-        lost = 36 * 2.0 ** -24 * scale * reach * (279 if dtype == torch.bfloat16 else 3 * 7)
-        share = 2 * abs(lost) + 2.0 ** -18 + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
-        tol = share * size + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) * want.abs()
+        wide = dtype == torch.float32
+        lost = 36 * 2.0 ** -24 * abs(scale) * reach * (3 * 7 if wide else 1039)
+        share = 2 * lost + 2.0 ** -18 + (0.0 if wide else 2.0 ** -8)
+        tol = share * size + (2.0 ** -24 if wide else 2.0 ** -8) * want.abs() + (0.0 if wide else 36 * 143 * 2.0 ** -24 * per_step)
         clear = ~spoilt
         assert bool(((got - want).abs() <= tol)[clear].all()), (r, ((got - want).abs() / tol.clamp_min(1e-30))[clear].max().item())
         t += n

@@ -33,7 +33,8 @@ def checks(monkeypatch):
     monkeypatch.setattr(ops, "_call", call)
     monkeypatch.setattr(ops, "_same_device", lambda what, *t: None)
     monkeypatch.setattr(ops, "_stream", lambda t: None)
-    monkeypatch.setattr(ops, "_kv4_room", lambda *a: (296, 8))
+    monkeypatch.setattr(ops, "_kv4_room", lambda *a: 296)
+    monkeypatch.setattr(ops, "_lib", lambda name: types.SimpleNamespace(lsb_attention_kv4_slot=lambda *a: 8))
 
 
 def _ctx(q_lens=(1, 3), kv_lens=(5, 3)):
