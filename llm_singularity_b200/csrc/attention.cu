@@ -78,6 +78,14 @@ struct RotatingParams : AttnParams {
     int rotary_dim, store;
 };
 
+// Windows that leave the keys before position `first` visible.
+struct FirstParams : AttnParams {
+    int first;
+};
+struct FirstSplitParams : SplitParams {
+    int first;
+};
+
 typedef unsigned long long pair32;              // two 32-bit values
 __device__ __forceinline__ pair32 twice(float a) {
     pair32 r;
@@ -174,10 +182,11 @@ static size_t single_smem(int hd, int heads, bool rotates) {
     return ((size_t)KT * (hd + 4) + (size_t)KT * hd + (size_t)heads * hd * 2 + (size_t)heads * (KT + 4) + heads * 4 + (rotates ? 2 * (size_t)hd : 0)) * 4;
 }
 
-// P: AttnParams, or RotatingParams to rotate and store.
+// P: AttnParams, RotatingParams to rotate and store, or FirstParams: the keys in reach are then counted without the gap between the
+// first tokens and the window, and stretches and tiles are of that count.
 template <typename T, int KT, int HDC, typename P>
 __global__ void __launch_bounds__(kThreads, 2) attention_single_kernel(const P p) {
-    constexpr bool ROTATES = std::is_same<P, RotatingParams>::value;
+    constexpr bool ROTATES = std::is_same<P, RotatingParams>::value, FIRST = std::is_same<P, FirstParams>::value;
     extern __shared__ __align__(16) float sm[];
     __shared__ long long off[2][KT];
     __shared__ float cs[2][ROTATES ? kMaxHeadDim / 2 : 1];     // cosines and sines of the token's position
@@ -203,9 +212,13 @@ __global__ void __launch_bounds__(kThreads, 2) attention_single_kernel(const P p
     float* fresh = ml + p.heads * 4;                           // the token's own key and value
     const int pos = p.kv_len[r] - 1;
     const int lo = (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0;
+    int few = 0;                                               // first tokens in front of the window
+    if constexpr (FIRST) few = min(p.first, lo);
+    const int from = FIRST ? 0 : lo, upto = FIRST ? few + pos - lo + 1 : pos + 1;
+    auto key_at = [&](int i) { return !FIRST ? i : i < few ? i : i - few + lo; };
     // this block's stretch: whole sixteens of keys
-    const int per = ((pos - lo + 1 + splits - 1) / splits + 15) / 16 * 16;
-    const int first = lo + split * per, last = min(pos + 1, first + per);     // [first, last), maybe empty
+    const int per = ((upto - from + splits - 1) / splits + 15) / 16 * 16;
+    const int first = from + split * per, last = min(upto, first + per);      // [first, last), maybe empty
     const int* table = p.block_table + (size_t)p.table_rows[r] * p.table_stride;
 
     const T* token = reinterpret_cast<const T*>(p.qkv) + (size_t)t * p.qkv_stride;
@@ -219,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_single_kernel(const P p
         for (int i = tid; i < H * hd; i += kThreads) qs[i] = lsb_to_float(token[(size_t)h0 * hd + i]) * p.scale;
     }
     if (tid < H) { ml[4 * tid] = -FLT_MAX; ml[4 * tid + 1] = 0.f; }
-    if (tid < KT) off[0][tid] = first + tid < last ? key_offset(p, table, g, first + tid) : -1;
+    if (tid < KT) off[0][tid] = first + tid < last ? key_offset(p, table, g, key_at(first + tid)) : -1;
     float acc[kAccs];
 #pragma unroll
     for (int a = 0; a < kAccs; ++a) acc[a] = 0.f;
@@ -267,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_single_kernel(const P p
             }
         }
         const int next = base + KT;
-        if (tid < KT) off[turn ^ 1][tid] = next + tid < last ? key_offset(p, table, g, next + tid) : -1;
+        if (tid < KT) off[turn ^ 1][tid] = next + tid < last ? key_offset(p, table, g, key_at(next + tid)) : -1;
         __syncthreads();
         if (next < last) tile.fetch(p, off[turn ^ 1], tid);
         for (int i = tid; i < H * KT; i += kThreads) {         // a (head, key) each: whole warps share a head
@@ -288,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_single_kernel(const P p
                 float s00, s01, s10, s11;
                 apart(s0, s00, s01);
                 apart(s1, s10, s11);
-                s = modified(p, (s00 + s01) + (s10 + s11), p.slopes ? p.slopes[h0 + h] : 0.f, pos - (base + k));
+                s = modified(p, (s00 + s01) + (s10 + s11), p.slopes ? p.slopes[h0 + h] : 0.f, pos - key_at(base + k));
             }
             ps[h * lds + k] = s;
         }
@@ -367,11 +380,12 @@ static size_t portion_smem(int hd) {
     return ((size_t)kRows * (hd + 4) + (size_t)KT * (hd + 4) + (size_t)KT * hd + (size_t)kRows * (KT + 4)) * 4;
 }
 
-// P: AttnParams, or SplitParams where a cluster of p.splits blocks shares out the keys of its rows.  (One kernel for both: 500
+// P: AttnParams, SplitParams where a cluster of p.splits blocks shares out the keys of its rows, or FirstSplitParams (as for single
+// tokens).  (One kernel for both: 500
 // tokens at 4,000 keys, 32 / 8 heads of 64 in 32-bit, whole, 746 us where it takes 691.)
 template <typename T, int KT, int HDC, typename P>
 __global__ void __launch_bounds__(kThreads, HDC <= 128 ? 2 : 1) attention_portion_kernel(const P p) {
-    constexpr bool SPLIT = std::is_same<P, SplitParams>::value;
+    constexpr bool FIRST = std::is_same<P, FirstSplitParams>::value, SPLIT = FIRST || std::is_same<P, SplitParams>::value;
     constexpr int KPT = KT / 16;                // keys of a thread's scores
     constexpr int CPT = HDC / 64;               // groups of four columns of a thread's sums
     extern __shared__ __align__(16) float sm[];
@@ -398,7 +412,11 @@ __global__ void __launch_bounds__(kThreads, HDC <= 128 ? 2 : 1) attention_portio
     const int pos0 = p.kv_len[r] - q_len + i0;                 // of the block's first query
     const int pos_last = min(pos0 + queries, p.kv_len[r]) - 1;
     // this block's tiles: every splits-th
-    const int lo = ((p.window > 0 && pos0 - p.window + 1 > 0) ? pos0 - p.window + 1 : 0) + split * KT, stride = SPLIT ? splits * KT : KT;
+    const int near = (p.window > 0 && pos0 - p.window + 1 > 0) ? pos0 - p.window + 1 : 0;
+    int few = 0;                                               // first tokens in front of the window
+    if constexpr (FIRST) few = min(p.first, near);
+    const int lo = (FIRST ? 0 : near) + split * KT, stride = SPLIT ? splits * KT : KT, end = FIRST ? few + pos_last - near : pos_last;
+    auto key_at = [&](int i) { return !FIRST ? i : i < few ? i : i - few + near; };
     const int* table = p.block_table + (size_t)p.table_rows[r] * p.table_stride;
 
     // row x: query i0 + x / heads, head h0 + x % heads (rows beyond the portion or the group stay zero)
@@ -408,10 +426,14 @@ __global__ void __launch_bounds__(kThreads, HDC <= 128 ? 2 : 1) attention_portio
             ? lsb_to_float(reinterpret_cast<const T*>(p.qkv)[(size_t)(qs0 + qi) * p.qkv_stride + (size_t)(h0 + h) * hd + d]) * p.scale
             : 0.f;
     }
-    if (tid < KT) off[0][tid] = lo + tid <= pos_last ? key_offset(p, table, g, lo + tid) : -1;
+    if (tid < KT) off[0][tid] = lo + tid <= end ? key_offset(p, table, g, key_at(lo + tid)) : -1;
     if (p.slopes && tid < kRows) slopes[tid] = tid % p.heads < H ? p.slopes[h0 + tid % p.heads] : 0.f;
     // (a row sees the keys whose distance is below this: one unsigned comparison for both of its ends)
     const unsigned reach = p.window > 0 ? (unsigned)p.window : 0x7fffffffu;
+    auto sees = [&](int at, int key) {
+        if constexpr (FIRST) return (unsigned)(at - key) < reach || (key < p.first && key <= at);
+        return (unsigned)(at - key) < reach;
+    };
     int pos[4];
     float m[4], l[4];
     pair32 acc[4][2 * CPT];
@@ -427,12 +449,12 @@ __global__ void __launch_bounds__(kThreads, HDC <= 128 ? 2 : 1) attention_portio
     __syncthreads();
     Tile<T, KT, HDC> tile;
     tile.fetch(p, off[0], tid);
-    for (int base = lo, turn = 0; base <= pos_last; base += stride, turn ^= 1) {
+    for (int base = lo, turn = 0; base <= end; base += stride, turn ^= 1) {
         const bool finite = tile.park(p, ks, vs, ldk, tid);
         const int next = base + stride;
-        if (tid < KT) off[turn ^ 1][tid] = next + tid <= pos_last ? key_offset(p, table, g, next + tid) : -1;
+        if (tid < KT) off[turn ^ 1][tid] = next + tid <= end ? key_offset(p, table, g, key_at(next + tid)) : -1;
         const bool by_row = __syncthreads_or(!finite);
-        if (next <= pos_last) tile.fetch(p, off[turn ^ 1], tid);
+        if (next <= end) tile.fetch(p, off[turn ^ 1], tid);
         // scores: rows 4 ty + i, keys tx + 16 j
         pair32 s2[4][KPT];
 #pragma unroll
@@ -462,10 +484,10 @@ __global__ void __launch_bounds__(kThreads, HDC <= 128 ? 2 : 1) attention_portio
             const float slope = p.slopes ? slopes[ty * 4 + i] : 0.f;
 #pragma unroll
             for (int j = 0; j < KPT; ++j) {
-                const int key = base + tx + 16 * j;
+                const int key = key_at(base + tx + 16 * j);
                 float u, v;
                 apart(s2[i][j], u, v);
-                seen[j] = (unsigned)(pos[i] - key) < reach && off[turn][tx + 16 * j] >= 0;
+                seen[j] = sees(pos[i], key) && off[turn][tx + 16 * j] >= 0;
                 s[j] = seen[j] ? modified(p, u + v, slope, pos[i] - key) : -FLT_MAX;
                 mx = fmaxf(mx, s[j]);
             }
@@ -495,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, HDC <= 128 ? 2 : 1) attention_portio
                 if (off[turn][k] < 0) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if ((unsigned)(pos[i] - (base + k)) >= reach) continue;
+                    if (!sees(pos[i], key_at(base + k))) continue;
                     const pair32 we = twice(ps[(ty * 4 + i) * ldp + k]);
 #pragma unroll
                     for (int c = 0; c < CPT; ++c) {
@@ -706,8 +728,8 @@ LSB_API int lsb_portion_splits(int hd, int nh, int nkv, int portions, int max_q_
 
 // rot: null, or the rotation of single tokens
 template <typename T, int KT, int HDC>
-static int launch(AttnParams p, const RotatingParams* rot, int n_requests, int max_q_len, int n_single, int max_keys, int portion_keys,
-                  cudaStream_t stream) {
+static int launch(AttnParams p, const RotatingParams* rot, int first, int n_requests, int max_q_len, int n_single, int max_keys,
+                  int portion_keys, cudaStream_t stream) {
     static int configured = -1;
     const int group = p.nh / p.nkv;
     if (configured < 0) {
@@ -717,6 +739,8 @@ static int launch(AttnParams p, const RotatingParams* rot, int n_requests, int m
         if (!rc) rc = allow(attention_single_kernel<T, KT, HDC, RotatingParams>);
         if (!rc) rc = allow(attention_portion_kernel<T, KT, HDC, AttnParams>);
         if (!rc) rc = allow(attention_portion_kernel<T, KT, HDC, SplitParams>);
+        if (!rc) rc = allow(attention_single_kernel<T, KT, HDC, FirstParams>);
+        if (!rc) rc = allow(attention_portion_kernel<T, KT, HDC, FirstSplitParams>);
         configured = rc;
     }
     if (configured) return configured;
@@ -735,7 +759,12 @@ static int launch(AttnParams p, const RotatingParams* rot, int n_requests, int m
         const dim3 grid((unsigned)splits, p.nkv * s.head_blocks, n_requests);
         const size_t smem = single_smem<KT>(p.hd, s.heads, rot != nullptr);
         int rc;
-        if (rot) {
+        if (first > 0) {
+            FirstParams with;
+            static_cast<AttnParams&>(with) = s;
+            with.first = first;
+            rc = launch_clusters(attention_single_kernel<T, KT, HDC, FirstParams>, grid, smem, (unsigned)splits, with, stream);
+        } else if (rot) {
             RotatingParams turned = *rot;
             static_cast<AttnParams&>(turned) = s;
             rc = launch_clusters(attention_single_kernel<T, KT, HDC, RotatingParams>, grid, smem, (unsigned)splits, turned, stream);
@@ -753,6 +782,13 @@ static int launch(AttnParams p, const RotatingParams* rot, int n_requests, int m
         const int splits = splits_of_portions<T, KT, HDC>(p.hd, p.nh, p.nkv, n_requests > n_single ? n_requests - n_single : 1, max_q_len, portion_keys, p.window);
         if (tiles * splits > 0x7fffffffll) return (int)cudaErrorInvalidValue;
         const dim3 grid((unsigned)(tiles * splits), p.nkv * p.head_blocks, n_requests);
+        if (first > 0) {
+            FirstSplitParams with;
+            static_cast<AttnParams&>(with) = p;
+            with.splits = splits;
+            with.first = first;
+            return launch_clusters(attention_portion_kernel<T, KT, HDC, FirstSplitParams>, grid, portion_smem<KT>(p.hd), (unsigned)splits, with, stream);
+        }
         if (splits == 1) return lsb_launch(attention_portion_kernel<T, KT, HDC, AttnParams>, grid, dim3(kThreads), portion_smem<KT>(p.hd), stream, 1, p);
         SplitParams parts;
         static_cast<AttnParams&>(parts) = p;
@@ -767,27 +803,51 @@ static int launch(AttnParams p, const RotatingParams* rot, int n_requests, int m
 // the launch is captured).
 // inv_freq: null, or the rotation of single tokens (float [rotary_dim / 2]), which come unrotated then, keys and values behind the
 // queries in their rows; `store`: and not yet in their pages.
-LSB_API int lsb_paged_attention_generic(
+static int paged_attention_generic(
     const void* qkv, int qkv_stride, const void* k_pages, const void* v_pages,
     const int* q_start, const int* kv_len, const int* table_rows, const int* block_table,
     int table_stride, void* out, int dtype, int n_requests, int max_q_len, int n_single, int max_keys, int portion_keys,
     int nh, int nkv, int hd, int page_size, int num_pages, float scale, int window,
-    float softcap, const float* slopes, const float* inv_freq, int rotary_dim, int store, cudaStream_t stream) {
+    float softcap, const float* slopes, const float* inv_freq, int rotary_dim, int store, int first, cudaStream_t stream) {
     if (n_requests <= 0 || max_q_len <= 0) return 0;
     if (hd % 16 || hd <= 0 || hd > kMaxHeadDim || nkv <= 0 || nh % nkv) return (int)cudaErrorInvalidValue;
     if (n_requests > 65535 || nh > 65535) return (int)cudaErrorInvalidValue;
     if (inv_freq && (rotary_dim < 0 || rotary_dim > hd || rotary_dim % 2 || qkv_stride < (nh + 2 * nkv) * hd)) return (int)cudaErrorInvalidValue;
     const AttnParams p{qkv, qkv_stride, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out,
                        nh, nkv, hd, page_size, num_pages, scale, window, softcap, slopes, 0, 0};
+    if (first < 0 || (first > 0 && (window <= 0 || inv_freq))) return (int)cudaErrorInvalidValue;
     RotatingParams rot;
     rot.inv_freq = inv_freq;
     rot.rotary_dim = rotary_dim;
     rot.store = store;
     const RotatingParams* rotation = inv_freq ? &rot : nullptr;
     LSB_DISPATCH_DTYPE(dtype, {
-        if (hd <= 64) return launch<T, 64, 64>(p, rotation, n_requests, max_q_len, n_single, max_keys, portion_keys, stream);
-        if (hd <= 128) return launch<T, 32, 128>(p, rotation, n_requests, max_q_len, n_single, max_keys, portion_keys, stream);
-        return launch<T, 32, 256>(p, rotation, n_requests, max_q_len, n_single, max_keys, portion_keys, stream);
+        if (hd <= 64) return launch<T, 64, 64>(p, rotation, first, n_requests, max_q_len, n_single, max_keys, portion_keys, stream);
+        if (hd <= 128) return launch<T, 32, 128>(p, rotation, first, n_requests, max_q_len, n_single, max_keys, portion_keys, stream);
+        return launch<T, 32, 256>(p, rotation, first, n_requests, max_q_len, n_single, max_keys, portion_keys, stream);
     });
     return 0;
+}
+
+LSB_API int lsb_paged_attention_generic(
+    const void* qkv, int qkv_stride, const void* k_pages, const void* v_pages,
+    const int* q_start, const int* kv_len, const int* table_rows, const int* block_table,
+    int table_stride, void* out, int dtype, int n_requests, int max_q_len, int n_single, int max_keys, int portion_keys,
+    int nh, int nkv, int hd, int page_size, int num_pages, float scale, int window,
+    float softcap, const float* slopes, const float* inv_freq, int rotary_dim, int store, cudaStream_t stream) {
+    return paged_attention_generic(qkv, qkv_stride, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out, dtype,
+                                   n_requests, max_q_len, n_single, max_keys, portion_keys, nh, nkv, hd, page_size, num_pages, scale, window,
+                                   softcap, slopes, inv_freq, rotary_dim, store, 0, stream);
+}
+
+// The same with the keys before position `first` beside the window's (single tokens come rotated and stored).
+LSB_API int lsb_paged_attention_generic_first(
+    const void* qkv, int qkv_stride, const void* k_pages, const void* v_pages,
+    const int* q_start, const int* kv_len, const int* table_rows, const int* block_table,
+    int table_stride, void* out, int dtype, int n_requests, int max_q_len, int n_single, int max_keys, int portion_keys,
+    int nh, int nkv, int hd, int page_size, int num_pages, float scale, int window,
+    float softcap, const float* slopes, int first, cudaStream_t stream) {
+    return paged_attention_generic(qkv, qkv_stride, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out, dtype,
+                                   n_requests, max_q_len, n_single, max_keys, portion_keys, nh, nkv, hd, page_size, num_pages, scale, window,
+                                   softcap, slopes, nullptr, 0, 0, first, stream);
 }

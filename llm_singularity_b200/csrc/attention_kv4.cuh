@@ -977,11 +977,11 @@ static int kv4_attention(const void* qkv, int qkv_stride, const void* pages, con
     LSB_API int lsb_attention_kv4(const void* qkv, int qkv_stride, const void* pages, const int* q_start, const int* kv_len, \
                                   const int* table_rows, const int* block_table, int table_stride, void* out, int n_requests, \
                                   long long max_rows, int nh, int nkv, int hd, int page_size, int num_pages, float scale,   \
-                                  int window, int first, int mode, int eights, int splits, int spread, float* parts,        \
-                                  cudaStream_t stream) {                                                                     \
+                                  int window, int first, int mode, int eights, int splits, int spread,     \
+                                  float* parts, cudaStream_t stream) {                                                       \
         return kv4_attention<T>(qkv, qkv_stride, pages, q_start, kv_len, table_rows, block_table, table_stride, out,         \
-                                n_requests, max_rows, nh, nkv, hd, page_size, num_pages, scale, window, first, mode, eights, \
-                                splits, spread, parts, stream);                                                              \
+                                n_requests, max_rows, nh, nkv, hd, page_size, num_pages, scale, window, first, mode,         \
+                                eights, splits, spread, parts, stream);                                                      \
     }                                                                                                                        \
     LSB_API int lsb_attention_kv4_room(int hd, int eights) {                                                                 \
         const int got = kv4_of<T>(hd, eights, Kv4Room{});                                                                    \

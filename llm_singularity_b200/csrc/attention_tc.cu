@@ -132,7 +132,10 @@ __device__ __forceinline__ int div_page(int key, int page_size, int page_shift) 
 #ifndef LSB_DEC_MINBLOCKS
 #define LSB_DEC_MINBLOCKS 4
 #endif
-template <int HD, bool LOW8, int STAGES>
+// One parameter more (a parameter pack, so that the others' kernel stays as it is): the keys before position `first` are seen
+// beside the window's; their chunks stand in front of the window's in the list that splits and warps share out, and no page in
+// between is looked at.
+template <int HD, bool LOW8, int STAGES, typename... First>
 __global__ void __launch_bounds__(kThreads, HD == 64 ? LSB_DEC_MINBLOCKS : 3)
 decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
                         bf16* k_pages, bf16* v_pages,
@@ -141,7 +144,10 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
                         int table_stride, bf16* __restrict__ out, float* __restrict__ part_o,
                         float* __restrict__ part_ml, int nh, int nkv, int page_size, int num_pages,
                         float scale, int window, int splits, int cluster_merge,
-                        const float* __restrict__ inv_freq, int rotary_dim, int store_kv, int longest_first) {
+                        const float* __restrict__ inv_freq, int rotary_dim, int store_kv, int longest_first, First... with_first) {
+    constexpr bool FIRST = sizeof...(First) == 1;
+    int first = 0;
+    if constexpr (FIRST) first = (with_first, ...);
     constexpr int CPR = HD / 8, KS = HD / 16;
     constexpr int kStageElems = 2 * kChunk * HD;             // K rows then V rows
     extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -180,7 +186,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
         const uint32_t key = t < n ? (uint32_t)own.z << 7 | (127 - t) : 0u;      // no two alike; equal lengths in their order
         keys[t] = key;
         // (what requests walk, a window at most)
-        const int seen = window > 0 ? min(own.z, window) : own.z;
+        const int seen = window > 0 ? min(own.z, FIRST ? window + first : window) : own.z;
         const int most = __reduce_max_sync(0xffffffffu, seen), least = __reduce_min_sync(0xffffffffu, seen > 0 ? seen : 0x7fffffff);
         if ((t & 31) == 0) { ends[t >> 5][0] = most; ends[t >> 5][1] = least; }
         if (t == r) chosen = own;
@@ -217,15 +223,28 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
     const int page_shift = (page_size & (page_size - 1)) == 0 ? __ffs(page_size) - 1 : -1;
 
     const int first_chunk = lo / kChunk;
-    const int n_chunks = p / kChunk + 1 - first_chunk;
+    int n_chunks = p / kChunk + 1 - first_chunk, front = 0, chunk0 = first_chunk;
+    if constexpr (FIRST) {
+        front = min((first + kChunk - 1) / kChunk, first_chunk);           // chunks of first tokens
+        n_chunks += front;
+        chunk0 = 0;
+    }
     const int per = (n_chunks + splits - 1) / splits;
-    const int c0 = first_chunk + split * per;
-    const int c1 = min(c0 + per, first_chunk + n_chunks);
+    const int c0 = chunk0 + split * per;
+    const int c1 = min(c0 + per, chunk0 + n_chunks);
+    auto chunk_at = [&](int c) {
+        if constexpr (FIRST) return c < front ? c : c - front + first_chunk;
+        else return c;
+    };
+    auto in_reach = [&](int key) {
+        if constexpr (FIRST) return (key >= lo || key < first) && key <= p;
+        else return key >= lo && key <= p;
+    };
 
     // this block's slice of the block table
     const int page0 = div_page(c0 * kChunk, page_size, page_shift);
     const int n_pages_here = c1 > c0 ? div_page(c1 * kChunk - 1, page_size, page_shift) - page0 + 1 : 0;
-    const bool cached = n_pages_here <= kBtCache;
+    const bool cached = !FIRST && n_pages_here <= kBtCache;  // (FIRST: in two pieces, looked up one by one)
     const int half = rotary_dim >> 1;                        // rotated pairs: dims (i, i + half), i < half
     if (inv_freq && single)
         for (int i = threadIdx.x; i < half; i += kThreads)
@@ -240,7 +259,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
     const int n_mine = (c1 - c0 - warp + 3) / 4;             // chunks c0 + warp, c0 + warp + 4, ...
     auto issue = [&](int i) {
         if (i < n_mine) {
-            const int chunk = c0 + warp + 4 * i;
+            const int chunk = chunk_at(c0 + warp + 4 * i);
             bf16* dK = ring + (size_t)(i % STAGES) * kStageElems;
             bf16* dV = dK + kChunk * HD;
             if (page_shift >= 0 && page_size >= kChunk) {
@@ -257,7 +276,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
 #pragma unroll
                 for (int idx = lane; idx < kChunk * CPR; idx += 32) {
                     const int kk = idx / CPR, c = idx - kk * CPR;
-                    const bool valid = page_ok && key0 + kk >= lo && key0 + kk <= p;
+                    const bool valid = page_ok && in_reach(key0 + kk);
                     const int off = valid ? idx * 8 : 0;
                     cp_async16(tile_ptr<HD>(dK, kk, c), srcK + off, valid);
                     cp_async16(tile_ptr<HD>(dV, kk, c), srcV + off, valid);
@@ -267,7 +286,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
             for (int idx = lane; idx < kChunk * CPR; idx += 32) {
                 const int kk = idx / CPR, c = idx - kk * CPR;
                 const int key = chunk * kChunk + kk;
-                bool valid = key >= lo && key <= p;
+                bool valid = in_reach(key);
                 long long off = 0;
                 if (valid) {
                     const int pi = div_page(key, page_size, page_shift);
@@ -384,7 +403,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
         issue(i + STAGES - 1);
         cp_async_wait<STAGES - 1>();
         __syncwarp();
-        const int chunk = c0 + warp + 4 * i;
+        const int chunk = chunk_at(c0 + warp + 4 * i);
         bf16* tK = ring + (size_t)(i % STAGES) * kStageElems;
         bf16* tV = tK + kChunk * HD;
 
@@ -407,7 +426,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
         constexpr int NE = 2 * NR;
         float mx[2] = {-INFINITY, -INFINITY};
         const int key0 = chunk * kChunk;
-        if (key0 >= lo && key0 + kChunk - 1 <= p) {            // whole chunk in range: no mask
+        if ((key0 >= lo || (FIRST && key0 + kChunk <= first)) && key0 + kChunk - 1 <= p) {      // whole chunk in range: no mask
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -422,7 +441,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
                     const int key = key0 + nt * 8 + 2 * (lane & 3) + (e & 1);
-                    const float v = (key >= lo && key <= p) ? s[nt][e] * sc : -INFINITY;
+                    const float v = in_reach(key) ? s[nt][e] * sc : -INFINITY;
                     s[nt][e] = v;
                     mx[e >> 1] = fmaxf(mx[e >> 1], v);
                 }
@@ -519,7 +538,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
         }
         const int head = g * G + h;
         if (splits == 1) {
-            out[(size_t)qs * nh * HD + (size_t)head * HD + d] = __float2bfloat16_rn(L > 0.f ? O / L : 0.f);
+            out[(size_t)qs * nh * HD + (size_t)head * HD + d] = __float2bfloat16_rn((FIRST ? L != 0.f : L > 0.f) ? O / L : 0.f);
         } else if (cluster_merge) {
             sFin[idx] = O;
             if (d == 0) { sFinML[2 * h] = M; sFinML[2 * h + 1] = L; }
@@ -546,7 +565,7 @@ decode_attention_kernel(const bf16* __restrict__ qkv, int qkv_stride,
                 L += ld_peer_f32(sFinML + 2 * h + 1, (uint32_t)s2) * f;
                 O += ld_peer_f32(sFin + idx, (uint32_t)s2) * f;
             }
-            out[(size_t)qs * nh * HD + (size_t)(g * G + h) * HD + d] = __float2bfloat16_rn(L > 0.f ? O / L : 0.f);
+            out[(size_t)qs * nh * HD + (size_t)(g * G + h) * HD + d] = __float2bfloat16_rn((FIRST ? L != 0.f : L > 0.f) ? O / L : 0.f);
         }
         cluster_barrier();          // nobody leaves while a peer may still read its shared memory
     }
@@ -824,6 +843,10 @@ template <int HD> static int configure_once() {
     if (e == cudaSuccess) e = allow_decode_smem<HD, true, kDeepStages<HD>>();
     if (e == cudaSuccess) e = allow_decode_smem<HD, false, kDeepStages<HD>>();
     if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(decode_attention_kernel<HD, true, kDecStages, int>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD>());
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(decode_attention_kernel<HD, false, kDecStages, int>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)decode_smem<HD>());
+    if (e == cudaSuccess)
         e = cudaFuncSetAttribute(prefill_attention_kernel<HD>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prefill_smem<HD>());
     done = (int)e;
@@ -975,6 +998,34 @@ LSB_API int lsb_decode_attention(const void* qkv, int qkv_stride, const void* k_
     return decode_launch(qkv, qkv_stride, const_cast<void*>(k_pages), const_cast<void*>(v_pages), q_start,
                          kv_len, table_rows, block_table, table_stride, out, scratch, n_requests, nh, nkv,
                          hd, page_size, num_pages, scale, window, splits, nullptr, 0, 0, 0, false, stream);
+}
+
+// With the keys before position `first` beside the window's.  At most as many splits as blocks of a portable cluster.
+LSB_API int lsb_decode_attention_first(const void* qkv, int qkv_stride, const void* k_pages, const void* v_pages,
+                                       const int* q_start, const int* kv_len, const int* table_rows,
+                                       const int* block_table, int table_stride, void* out, int n_requests, int nh, int nkv,
+                                       int hd, int page_size, int num_pages, float scale, int window, int splits, int first,
+                                       cudaStream_t stream) {
+    if (n_requests <= 0) return 0;
+    if (nkv <= 0 || nh % nkv || nh / nkv > 16 || splits < 1 || splits > 8 || n_requests > 65535 || nkv > 65535 || window <= 0 || first < 0)
+        return (int)cudaErrorInvalidValue;
+    const dim3 grid(splits, nkv, n_requests);
+    const bool low8 = nh / nkv <= 8;
+#define LAUNCH_FIRST(HD)                                                                                                  \
+    do {                                                                                                                  \
+        if (const int rc = configure_once<HD>()) return rc;                                                               \
+        const bool ordered = splits == 1 && n_requests <= kThreads &&                                                     \
+                             (long long)n_requests * nkv > (long long)lsb_decode_blocks_per_sm(HD, nh / nkv) * num_sms(); \
+        return lsb_launch(low8 ? decode_attention_kernel<HD, true, kDecStages, int> : decode_attention_kernel<HD, false, kDecStages, int>, grid, \
+                          dim3(kThreads), decode_smem<HD>(), stream, splits, (const bf16*)qkv, qkv_stride, (bf16*)const_cast<void*>(k_pages), \
+                          (bf16*)const_cast<void*>(v_pages), q_start, kv_len, table_rows, block_table, table_stride, (bf16*)out, \
+                          (float*)nullptr, (float*)nullptr, nh, nkv, page_size, num_pages, scale, window, splits,          \
+                          splits > 1 ? 1 : 0, (const float*)nullptr, 0, 0, ordered ? 1 : 0, first);                        \
+    } while (0)
+    if (hd == 64) LAUNCH_FIRST(64);
+    if (hd == 128) LAUNCH_FIRST(128);
+#undef LAUNCH_FIRST
+    return (int)cudaErrorInvalidValue;
 }
 
 // The same over a projection that has not been rotated yet: the kernel rotates the queries and the

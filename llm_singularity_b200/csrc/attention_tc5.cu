@@ -16,12 +16,15 @@
 // block's softmax overlaps the other's matrix products.  All mbarrier waits are bounded.
 //
 // Query row i of a request with q_len new tokens and kv_len cached tokens sits at position
-// p = kv_len - q_len + i and sees keys [max(0, p - window + 1), p].  This kernel takes what the
+// p = kv_len - q_len + i and sees keys [max(0, p - window + 1), p], and with `first` also those of [0, min(first, p + 1)):
+// the tiles that hold them are walked in front of the window's, those between are not.  This kernel takes what the
 // reference's paged_attention_kernel (kernels/src/attention.cu:27-172) does one row at a time during
 // prefill (models/llama/llama_model.cpp:599-615).  No load in this file uses cluster multicast.
 #include "common.cuh"
 
 #include <cuda.h>
+
+#include <type_traits>
 
 LSB_DEFINE_STATUS()
 
@@ -50,6 +53,12 @@ struct AttnParams {
     int linear_bias;              // head h's score for a key d positions back loses 2^(-8 (h + 1) / nh) * d
 };
 
+// Windows that leave a request's first tokens visible.  (Parameters of their own, as in attention.cu: behind those of every launch
+// they would make the others slower.)
+struct FirstParams : AttnParams {
+    int first;                    // keys before this position are seen by every row at or behind them
+};
+
 template <int HD>
 struct Smem {
     static constexpr int kKB = HD / 64;                     // 64-dim blocks of a head
@@ -74,10 +83,11 @@ struct Smem {
     static constexpr size_t kTotal = 1024 + kQBytes + 2 * kStages * kKVBytes + kBtCache * 4 + kBars * 8 + 16;
 };
 
-template <int HD>
+template <int HD, typename P>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 prefill_attention_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                             const __grid_constant__ CUtensorMap map_v, const AttnParams prm) {
+                             const __grid_constant__ CUtensorMap map_v, const P prm) {
+    constexpr bool FIRST = std::is_same<P, FirstParams>::value;
     using L = Smem<HD>;
     constexpr int KB = L::kKB;
     constexpr uint32_t kTmemCols = L::kTmemCols;
@@ -126,7 +136,16 @@ prefill_attention_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __
     const int pages_per_tile = kKeys >> prm.page_shift;
     const int page_first = (t0 * kKeys) >> prm.page_shift;
     const int page_last = p_last >> prm.page_shift;          // last page that holds a needed key
-    const int n_pages_here = page_last - page_first + 1;
+    int n_pages_here = page_last - page_first + 1;
+    // FIRST: tiles of first tokens stand in front of those from t0 on, and their pages in front of the others'
+    int first = 0, front = 0, front_pages = 0;
+    if constexpr (FIRST) {
+        first = prm.first;
+        front = min((first + kKeys - 1) / kKeys, t0);
+        front_pages = front * pages_per_tile;
+        n_pages_here += front_pages;
+    }
+    auto tile_of = [&](int t) { return FIRST && t < front ? t : t0 + t - front; };
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -149,21 +168,27 @@ prefill_attention_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __
     // Pages that lie wholly before the first key any row of this block may see (a window has passed
     // them) may have been given back already: their keys are masked, any page stands in for them.
     const int page_needed = lo_cta >> prm.page_shift;
-    for (int idx = threadIdx.x; idx < min(n_pages_here, kBtCache); idx += kThreads) {
-        int page = (page_first + idx < prm.table_stride) ? bt[page_first + idx] : -1;
+    // (FIRST: their place is taken by the block's last page, which its rows see.)
+    auto page_at = [&](int pi) {
+        int page = pi < prm.table_stride ? bt[pi] : -1;
+        if constexpr (FIRST) {
+            if (pi < page_needed && (long long)pi * prm.page_size >= first) page = page_last < prm.table_stride ? bt[page_last] : -1;
+        }
         if (page < 0 || page >= prm.num_pages) {
-            if (page_first + idx >= page_needed) lsb_set_status(LSB_BAD_PAGE);
+            if (FIRST || pi >= page_needed) lsb_set_status(LSB_BAD_PAGE);
             page = 0;
         }
-        sBT[idx] = page;
-    }
+        return page;
+    };
+    for (int idx = threadIdx.x; idx < min(n_pages_here, kBtCache); idx += kThreads)
+        sBT[idx] = page_at(FIRST && idx < front_pages ? idx : page_first + idx - front_pages);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_s = *tmem_slot;                      // S of even tiles, then of odd tiles
     const uint32_t tmem_p = tmem_s + L::kPCol;               // P of even tiles, then of odd tiles
     const uint32_t tmem_o = tmem_s + L::kOCol;               // O tile
-    const int n_tiles = t1 - t0;
+    const int n_tiles = t1 - t0 + front;
 
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
@@ -186,18 +211,10 @@ prefill_attention_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __
             // (each lane issues its page's copies: one elected lane for all of them was 10 % slower)
             if (lane < pages_per_tile) {
                 // pages past the last needed one repeat it: their keys are masked, their bytes finite
-                int pi = (((t0 + t) * kKeys) >> prm.page_shift) + lane;
+                int pi = ((tile_of(t) * kKeys) >> prm.page_shift) + lane;
                 if (pi > page_last) pi = page_last;
-                const int idx = pi - page_first;
-                int page;
-                if (idx < kBtCache) page = sBT[idx];
-                else {
-                    page = pi < prm.table_stride ? bt[pi] : -1;
-                    if (page < 0 || page >= prm.num_pages) {
-                        if (pi >= page_needed) lsb_set_status(LSB_BAD_PAGE);
-                        page = 0;
-                    }
-                }
+                const int idx = FIRST && t < front ? pi : pi - page_first + front_pages;
+                const int page = idx < kBtCache ? sBT[idx] : page_at(pi);
                 unsigned char* dst = stages + s * L::kKVBytes + lane * prm.page_size * 128;    // rows of a 64-dim block
                 for (int kb = 0; kb < KB; ++kb) tma_load_4d(dst + kb * (kKeys * 128), map, &full[s], kb * 64, 0, g, page);
                 if (!L::kShareS) tma_load_4d(dst + (sV - sK), &map_v, &full[s], 0, 0, g, page);
@@ -331,9 +348,9 @@ prefill_attention_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __
                     tmem_ld_32x32(tmem_s + lane_sel + (uint32_t)((t & 1) * kKeys + c0),
                                   *reinterpret_cast<uint32_t(*)[32]>(&v[c0]));
             }
-            const int key0 = (t0 + t) * kKeys;
+            const int key0 = tile_of(t) * kKeys;
             const bool full = key0 + kKeys - 1 <= p0 && rows == kRows &&
-                              (prm.window <= 0 || key0 > p_last - prm.window);
+                              (prm.window <= 0 || key0 > p_last - prm.window || (FIRST && key0 + kKeys <= first));
             // this tile's P buffer was read by the P V of the tile before the previous one
             // (where P shares S's columns, S of this tile was not formed before that)
             uint32_t p_free = 1;
@@ -367,6 +384,18 @@ prefill_attention_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll
                 for (int x = 0; x < kKeys; x += 2)
                     mxa[(x >> 1) & 3] = max3(mxa[(x >> 1) & 3], __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+            } else if constexpr (FIRST) {
+                // which keys, as bits: one test a key where comparisons with three ends would take three (a portion of 2,000 after
+                // 6,000, window 1,024, 32 / 8 heads of 64: 52 us, 71 with them)
+                auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; };
+                const uint64_t keep = below(c_hi + 1) & (~below(c_lo) | below(first - key0));
+                const uint32_t keep0 = (uint32_t)keep, keep1 = (uint32_t)(keep >> 32);
+#pragma unroll
+                for (int x = 0; x < kKeys; ++x) {
+                    const float sv = ((x < 32 ? keep0 : keep1) & (1u << (x & 31))) ? __uint_as_float(v[x]) : -INFINITY;
+                    v[x] = __float_as_uint(sv);
+                    mxa[x & 3] = fmaxf(mxa[x & 3], sv);
+                }
             } else {
 #pragma unroll
                 for (int x = 0; x < kKeys; ++x) {
@@ -497,29 +526,29 @@ LSB_API int lsb_prefill_attention_tc5_supported(const void* qkv, int qkv_stride,
            ((uintptr_t)v_pages % 16) == 0;
 }
 
-template <int HD>
-static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& prm,
+template <int HD, typename P>
+static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const P& prm,
                   dim3 grid, cudaStream_t stream) {
     static int configured = -1;
     constexpr size_t smem = Smem<HD>::kTotal;
     if (configured < 0)
-        configured = (int)cudaFuncSetAttribute(prefill_attention_tc5_kernel<HD>,
+        configured = (int)cudaFuncSetAttribute(prefill_attention_tc5_kernel<HD, P>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (configured) return configured;
-    return lsb_launch(prefill_attention_tc5_kernel<HD>, grid, dim3(kThreads), smem, stream, 1, mq, mk, mv, prm);
+    return lsb_launch(prefill_attention_tc5_kernel<HD, P>, grid, dim3(kThreads), smem, stream, 1, mq, mk, mv, prm);
 }
 
 // Every request of the step is processed (single decode tokens too, as 1-row tiles, unless
 // skip_single).
 // `softcap` > 0: a scaled score s becomes softcap * tanh(s / softcap); `linear_bias`: head h's score for a key d
 // positions back then loses 2^(-8 (h + 1) / nh) * d.
-LSB_API int lsb_prefill_attention_tc5_biased(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,
+static int prefill(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,
                                              const void* v_pages, const int* q_start, const int* kv_len,
                                              const int* table_rows, const int* block_table, int table_stride, void* out,
                                              int n_requests, int max_q_len, int nh, int nkv, int hd, int page_size,
                                              int num_pages, float scale, int window, int skip_single, int sink,
                                              const void* gate, long long gate_stride, float softcap, int linear_bias,
-                                             const float* sink_logit, cudaStream_t stream) {
+                                             const float* sink_logit, int first, cudaStream_t stream) {
     if (n_requests <= 0 || max_q_len <= 0) return 0;
     if (!lsb_prefill_attention_tc5_supported(qkv, qkv_stride, k_pages, v_pages, nh, nkv, hd, page_size) ||
         n_requests > 65535 || (max_q_len + kRows - 1) / kRows > 65535)
@@ -550,7 +579,37 @@ LSB_API int lsb_prefill_attention_tc5_biased(const void* qkv, int qkv_stride, in
     while ((1 << sh) < page_size) ++sh;
     prm.page_shift = sh;
     dim3 grid(nh, (max_q_len + kRows - 1) / kRows, n_requests);
+    if (first > 0 && window > 0) {
+        FirstParams with;
+        static_cast<AttnParams&>(with) = prm;
+        with.first = first;
+        return hd == 64 ? launch<64>(mq, mk, mv, with, grid, stream) : launch<128>(mq, mk, mv, with, grid, stream);
+    }
     return hd == 64 ? launch<64>(mq, mk, mv, prm, grid, stream) : launch<128>(mq, mk, mv, prm, grid, stream);
+}
+
+LSB_API int lsb_prefill_attention_tc5_biased(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,
+                                             const void* v_pages, const int* q_start, const int* kv_len,
+                                             const int* table_rows, const int* block_table, int table_stride, void* out,
+                                             int n_requests, int max_q_len, int nh, int nkv, int hd, int page_size,
+                                             int num_pages, float scale, int window, int skip_single, int sink,
+                                             const void* gate, long long gate_stride, float softcap, int linear_bias,
+                                             const float* sink_logit, cudaStream_t stream) {
+    return prefill(qkv, qkv_stride, n_tokens, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out,
+                   n_requests, max_q_len, nh, nkv, hd, page_size, num_pages, scale, window, skip_single, sink, gate, gate_stride,
+                   softcap, linear_bias, sink_logit, 0, stream);
+}
+
+// `first`: keys before this position stay visible beside the window's.
+LSB_API int lsb_prefill_attention_tc5_first(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,
+                                            const void* v_pages, const int* q_start, const int* kv_len,
+                                            const int* table_rows, const int* block_table, int table_stride, void* out,
+                                            int n_requests, int max_q_len, int nh, int nkv, int hd, int page_size,
+                                            int num_pages, float scale, int window, int skip_single, int first,
+                                            cudaStream_t stream) {
+    return prefill(qkv, qkv_stride, n_tokens, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out,
+                   n_requests, max_q_len, nh, nkv, hd, page_size, num_pages, scale, window, skip_single, 0, nullptr, 0, 0.f, 0,
+                   nullptr, first, stream);
 }
 
 LSB_API int lsb_prefill_attention_tc5(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,

@@ -220,6 +220,78 @@ __global__ void __launch_bounds__(256) read_kv4_kernel(const unsigned char* page
     for (int e = 0; e < 8; ++e) out[e] = lsb_from_float<T>(f[e]);
 }
 
+// What the portions of a step see of their 4-bit caches, as an ordinary cache in bfloat16 with pages of one tile, for the prompt
+// attention that reads its tiles as tensors: exact (kv4.cuh).  The tiles of first tokens and those from the oldest row's window on
+// stand side by side, so positions behind the gap are `gap` (a multiple of 16) less there: expanded[r] is the length that
+// the attention is to take request r for.  Tokens that are not there yet read as zeros (their weights are zeros, and zero times
+// what a page held before may be no number).
+// A block for each tile of a kv head; it moves 18 hd bytes in and 64 hd out.
+__global__ void __launch_bounds__(128) expand_kv4_kernel(const unsigned char* pages, const int* q_start, const int* kv_len, const int* table_rows,
+                                                         const int* block_table, int table_stride, __nv_bfloat16* k_out,
+                                                         __nv_bfloat16* v_out, int* table_out, int* rows_out, int* expanded,
+                                                         int room, int nkv, int hd, int page_size, int num_pages, int window, int first) {
+    // (The attention behind it reads lengths and rows before it waits, as a step's metadata may be read: it must not start before
+    // they are there, so this kernel lets nothing start early.)
+    const int c = blockIdx.x, h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x;
+    const int q_len = q_start[r + 1] - q_start[r], len = kv_len[r], p_lo = len - q_len;
+    const int near = (window > 0 && p_lo - window + 1 > 0 ? p_lo - window + 1 : 0) / kKv4Tile;
+    const int early = window > 0 ? min((first + kKv4Tile - 1) / kKv4Tile, near) : 0, gap = (near - early) * kKv4Tile;
+    const int place = r * room + c;
+    lsb_pdl_wait();
+    if (h == 0 && tid == 0) {
+        table_out[place] = place;
+        if (c == 0) {
+            expanded[r] = len - gap;
+            rows_out[r] = r;
+        }
+    }
+    const int pos0 = (c < early ? c : c - early + near) * kKv4Tile, pi = pos0 / page_size;
+    if (q_len == 1 || pos0 >= len) return;                              // (single tokens are another kernel's)
+    const int page = pi < table_stride ? block_table[(size_t)table_rows[r] * table_stride + pi] : -1;
+    const bool held = page >= 0 && page < num_pages;
+    if (!held && tid == 0) lsb_set_status(LSB_BAD_PAGE);
+    const unsigned char* tile = pages + (((size_t)(held ? page : 0) * nkv + h) * (page_size / kKv4Tile) + pos0 % page_size / kKv4Tile) * kv4_tile_bytes(hd);
+    const int per = hd / 8, G = hd / kKv4Group;
+    for (int i = tid; i < 2 * kKv4Tile * per; i += 128) {
+        const bool value = i >= kKv4Tile * per;
+        const int j = value ? i - kKv4Tile * per : i, t = j / per, d8 = j - t * per, g = d8 / 4;
+        uint4 packed = make_uint4(0, 0, 0, 0);
+        if (held && pos0 + t < len) {
+            uint32_t word;                                              // codes of dims 8 d8 .. 8 d8 + 7, in order
+            if (value) {
+                const unsigned char* v = tile + kv4_values_at(hd) + t * (hd / 2) + d8 / 2;
+                const int e = d8 % 2 * 4;
+                word = v[e * 2 * G] | v[(e + 1) * 2 * G] << 8 | v[(e + 2) * 2 * G] << 16 | (uint32_t)v[(e + 3) * 2 * G] << 24;
+            } else {
+                word = *reinterpret_cast<const uint32_t*>(tile + t * (hd / 2) + (d8 % 4 * G + g) * 4);
+            }
+            const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(
+                tile + (value ? kv4_value_scales_at(hd) : kv4_key_scales_at(hd)) + (t * G + g) * 2));
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn((float)((int)(word >> (8 * k) & 15u) - 8) * s,
+                                                               (float)((int)(word >> (8 * k + 4) & 15u) - 8) * s);
+                w[k] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+            packed = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>((value ? v_out : k_out) + (((size_t)place * nkv + h) * kKv4Tile + t) * hd + 8 * d8) = packed;
+    }
+}
+
+// `room`: tiles that each request has in k_out and v_out [requests * room, nkv, 16, hd]; table_out [requests, room].
+LSB_API int lsb_expand_kv4(const void* pages, const int* q_start, const int* kv_len, const int* table_rows, const int* block_table,
+                           int table_stride, void* k_out, void* v_out, int* table_out, int* rows_out, int* expanded,
+                           int n_requests, int room, int nkv, int hd, int page_size, int num_pages, int window, int first,
+                           cudaStream_t stream) {
+    if (n_requests <= 0 || room <= 0) return 0;
+    if (nkv > 65535 || n_requests > 65535) return (int)cudaErrorInvalidValue;
+    return lsb_launch(expand_kv4_kernel, dim3(room, nkv, n_requests), dim3(128), 0, stream, 1, (const unsigned char*)pages, q_start, kv_len,
+                      table_rows, block_table, table_stride, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, table_out, rows_out, expanded,
+                      room, nkv, hd, page_size, num_pages, window, first);
+}
+
 LSB_API int lsb_rope_kv4_store(const void* qkv, int dtype, int n_tokens, int nh, int nkv, int hd, const int* positions,
                                const int* token_req, const int* table_rows, const int* block_table, int table_stride,
                                const float* inv_freq, int rotary_dim, void* q_out, void* pages, int page_size, int num_pages,

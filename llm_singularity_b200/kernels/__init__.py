@@ -803,14 +803,14 @@ def _single_tokens_rotate(ctx, nh: int, nkv: int, hd: int, device) -> bool:
 def rope_store_attention(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache,
                          inv_freq: Optional[torch.Tensor], rotary_dim: int, store: bool,
                          scale: float, window: int, out: torch.Tensor, softcap: float = 0.0,
-                         slopes: Optional[torch.Tensor] = None) -> None:
+                         slopes: Optional[torch.Tensor] = None, first: int = 0) -> None:
     """``rope_kv_store`` followed by ``paged_attention``, as one operation.  Where the kernel of single
     tokens can do the rotation and the cache write itself (on the tensor cores with the rotated part
     of the head a multiple of 16 wide, the generic one with any; no score modifier), the separate kernel
-    runs only for the tokens of prompt portions, or not at all."""
-    if softcap or slopes is not None:
+    runs only for the tokens of prompt portions, or not at all (nor where first tokens stay visible)."""
+    if softcap or slopes is not None or (first and window):
         rope_kv_store(qkv, nh, nkv, hd, ctx, cache, inv_freq, rotary_dim, store)
-        paged_attention(qkv, nh, nkv, hd, ctx, cache, scale, window, out, softcap=softcap, slopes=slopes)
+        paged_attention(qkv, nh, nkv, hd, ctx, cache, scale, window, out, softcap=softcap, slopes=slopes, first=first)
         return
     on_tc = tensor_core_attention_ok(qkv.dtype, hd, nh, nkv)
     fuse = FUSE_DECODE_ROPE and 0 < rotary_dim <= hd and inv_freq is not None and (
@@ -849,8 +849,9 @@ def rope_store_attention(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cac
 def paged_attention(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, scale: float,
                     window: int, out: torch.Tensor, decode_rope=None, only: Optional[str] = None,
                     stream: Optional[int] = None, softcap: float = 0.0,
-                    slopes: Optional[torch.Tensor] = None) -> None:
-    """Causal attention of this step's query rows over their requests' cached keys and values.
+                    slopes: Optional[torch.Tensor] = None, first: int = 0) -> None:
+    """Causal attention of this step's query rows over their requests' cached keys and values: of a row at position p those at
+    positions j <= p with j > p - ``window`` (0: all) or j < ``first``.  Pages that hold neither are not looked at.
 
     Score modifiers: ``softcap`` > 0 replaces a scaled score s by ``softcap * tanh(s / softcap)``;
     ``slopes`` (float32 [heads]) subtracts ``slopes[h] * (query position - key position)``.  A
@@ -889,6 +890,13 @@ def paged_attention(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, s
             raise KernelError(f"attention: {slopes.shape[0]} slopes for {nh} heads")
     if softcap < 0:
         raise KernelError("attention: the soft cap must be positive (0: none)")
+    if first < 0:
+        raise KernelError("attention: the number of first tokens must not be negative (0: none)")
+    if first and window > 0:
+        if decode_rope is not None or only is not None or stream is not None:
+            raise KernelError("attention: beside first tokens, queries and keys come rotated and all requests go together")
+        _attention_with_first(qkv, nh, nkv, hd, ctx, cache, scale, window, min(first, 1 << 30), out, common, float(softcap), slopes)
+        return
     if modified or not tensor_core_attention_ok(qkv.dtype, hd, nh, nkv):
         if decode_rope is not None and modified:
             raise KernelError("attention: scores are modified where queries and keys come rotated")
@@ -1030,15 +1038,20 @@ def _kv4_room(lib: str, hd: int, eights: int, device) -> int:
 
 def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int, capacity: int, device) -> list:
     """The launches of a step's attention over a 4-bit cache, worked out once per step and kind of layer: (mode, offset into the
-    per-request arrays, requests, rows of a request, eights of rows of a block, blocks of a cluster, blocks of a spread launch, floats of
-    its parts).
+    per-request arrays, requests, rows of a request, eights of rows of a block, blocks of a cluster, blocks of a spread launch or
+    tiles of an expanded cache, floats of a spread launch's parts).
 
     Single tokens either have a cluster of blocks to each row tile, or are spread: equal stretches of all chunks of 32 tokens
     for as many blocks as fit, and a kernel that joins what was cut.  The first ends when the longest context has ended (and has rounds
     where blocks are more than fit), the second costs about 24 chunks a block more (measured, heads of 64 and 128 in bfloat16: 64
     requests of 1,000 - 8,100 tokens 147 us with clusters of one, 107 spread; 64 of 4,096 55 and 59; 8 of 4,096 18 and 23;
     one of 131,072 107 and 50).  A captured launch does not know the lengths: it is spread if the block tables have room for
-    long contexts."""
+    long contexts.
+
+    Portions of 128 tokens and more in bfloat16 with heads of 64 or 128 (mode 3) are expanded: what they see is unpacked once, to an
+    ordinary cache, for the tcgen05 prompt kernel (2,011 tokens after 4,096, 32 / 8 heads of 128: 1,000 us where every row tile unpacks
+    for itself, 229 us so), as long as that cache stays within 1 GB (256 MB in a captured step, which has to have room
+    for the longest context)."""
     key = (lib, nh, nkv, hd, window, first, capacity)
     plans = ctx.__dict__.setdefault("_kv4_plans", {})
     if key in plans:
@@ -1058,6 +1071,11 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
             seen = min(seen, window + most + first)
         chunks = -(-seen // 32)                     # the most of a row tile
         splits = spread = parts = 0
+        if mode == 2 and most >= 128 and lib == "attention_kv4" and hd in _TC_HEAD_DIMS and USE_TCGEN05_ATTENTION:
+            tiles_seen = -(-seen // 16) + 2         # (a window's first tile and the first tokens' last may be cut)
+            if count * tiles_seen * nkv * 64 * hd <= (1 << 28 if fixed else 1 << 30):
+                plan.append((3, 4 * at, count, rows, eights, 1, tiles_seen, 0))
+                continue
         cost = None
         for s in range(1, 9):
             rounds = -(-tiles * s // room)
@@ -1103,15 +1121,67 @@ def paged_attention_kv4(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cach
     _same_device("paged_attention_kv4", qkv, out, pages, table)
     if out.data_ptr() % 16:
         raise KernelError("paged_attention_kv4: out must start at a multiple of 16 bytes")
-    lib = "attention_kv4" if _dt(qkv) == _BF16 else "attention_kv4_f32"
-    window, first, width = min(window, 1 << 30), min(first, 1 << 30), table.shape[1]
+    lib, group = "attention_kv4" if _dt(qkv) == _BF16 else "attention_kv4_f32", nh // nkv
+    window, first, width = min(window, (1 << 30) - 1), min(first, 1 << 30), table.shape[1]
     q_start, kv_len, rows_of = ctx.q_start.data_ptr(), ctx.kv_len.data_ptr(), ctx.table_rows.data_ptr()
     for mode, off, count, rows, eights, splits, spread, parts in _kv4_plan(ctx, lib, nh, nkv, hd, window, first,
                                                                            width * cache.page_size, qkv.device):
-        scratch = torch.empty(parts, dtype=torch.float32, device=qkv.device) if spread else None
-        _call(lib, "lsb_attention_kv4", _p(qkv), ld, _p(pages), ctypes.c_void_p(q_start + off), ctypes.c_void_p(kv_len + off),
-              ctypes.c_void_p(rows_of + off), _p(table), width, _p(out), count, _ll(rows), nh, nkv, hd, cache.page_size,
-              pages.shape[0], _f(scale), window, first, mode, eights, splits, spread, _p(scratch), _stream(out))
+        per_request = (ctypes.c_void_p(q_start + off), ctypes.c_void_p(kv_len + off), ctypes.c_void_p(rows_of + off))
+        scratch = None
+        if mode == 3 and (scale <= 0 or ld % 8 or qkv.data_ptr() % 16):
+            mode, spread = 2, 0                     # (what the prompt kernel does not take)
+        if mode == 3:
+            room, dev = spread, qkv.device
+            kv = torch.empty(2, count * room, nkv, 16, hd, dtype=qkv.dtype, device=dev)
+            ints = torch.empty(count * (room + 2), dtype=torch.int32, device=dev)
+            its_table, its_rows, its_len = ints[:count * room], ints[count * room:count * (room + 1)], ints[count * (room + 1):]
+            _call("kv4_store", "lsb_expand_kv4", _p(pages), *per_request, _p(table), width, _p(kv[0]), _p(kv[1]), _p(its_table),
+                  _p(its_rows), _p(its_len), count, room, nkv, hd, cache.page_size, pages.shape[0], window, first, _stream(out))
+            _call("attention_tc5", "lsb_prefill_attention_tc5_first", _p(qkv), ld, T, _p(kv[0]), _p(kv[1]), per_request[0],
+                  _p(its_len), _p(its_rows), _p(its_table), room, _p(out), count, rows // group, nh, nkv, hd, 16, count * room,
+                  _f(scale), window, 1, first, _stream(out))
+            # (that kernel multiplies the zero weights of hidden places with what is there)
+            _call("attention_repair", "lsb_attention_repair", _p(qkv), ld, _p(pages), _p(None), *per_request, _p(table), width, _p(out),
+                  count, rows // group, nh, nkv, hd, cache.page_size, pages.shape[0], _f(scale), window, first, 1, _stream(out))
+            continue
+        if spread:
+            scratch = torch.empty(parts, dtype=torch.float32, device=qkv.device)
+        _call(lib, "lsb_attention_kv4", _p(qkv), ld, _p(pages), *per_request, _p(table), width, _p(out), count, _ll(rows), nh, nkv,
+              hd, cache.page_size, pages.shape[0], _f(scale), window, first, mode, eights, splits, spread, _p(scratch), _stream(out))
+
+
+def _attention_with_first(qkv, nh, nkv, hd, ctx, cache, scale, window, first, out, common, softcap, slopes) -> None:
+    """``paged_attention`` where first tokens stay visible.  On the tensor cores single tokens go to the split-KV kernel and
+    portions of any length to the tcgen05 one, whose blocks and tiles skip what lies between; else both to the generic kernels."""
+    window, R = min(window, (1 << 30) - 1), ctx.n_requests
+    fixed = getattr(ctx, "fixed_launch", False)
+    n_single, begin, end = _batch_shape(ctx)
+    longest, of_portions = (0, 0) if fixed else (min(ctx.max_kv_len, window + first), _portion_keys(ctx))
+    sizes = (_i(nh), _i(nkv), _i(hd), _i(cache.page_size), _i(cache.k_pages.shape[0]), _f(scale), _i(window))
+    on_tc = tensor_core_attention_ok(qkv.dtype, hd, nh, nkv) and not softcap and slopes is None
+    prompts = on_tc and USE_TCGEN05_ATTENTION and scale > 0 and qkv.shape[0] == ctx.n_tokens and out.data_ptr() % 16 == 0 \
+        and bool(_lib("attention_tc5").lsb_prefill_attention_tc5_supported(
+            _p(qkv), _i(qkv.shape[1]), _p(cache.k_pages), _p(cache.v_pages), _i(nh), _i(nkv), _i(hd), _i(cache.page_size)))
+    if n_single and on_tc:
+        splits = min(8, decode_splits(n_single, nkv, qkv.device, hd, nh // nkv))
+        if not fixed:
+            splits = min(splits, -(-longest // 128))
+        _call("attention_tc", "lsb_decode_attention_first", *common, _i(R), *sizes, _i(splits), _i(first), _stream(out))
+        n_single = 0
+    if begin < end and prompts:
+        off = 4 * begin
+        per_request = (ctypes.c_void_p(ctx.q_start.data_ptr() + off), ctypes.c_void_p(ctx.kv_len.data_ptr() + off),
+                       ctypes.c_void_p(ctx.table_rows.data_ptr() + off), _p(cache.block_table), _i(cache.block_table.shape[1]), _p(out),
+                       _i(end - begin), _i(ctx.max_q_len))
+        _call("attention_tc5", "lsb_prefill_attention_tc5_first", _p(qkv), _i(qkv.shape[1]), _i(ctx.n_tokens), _p(cache.k_pages),
+              _p(cache.v_pages), *per_request, *sizes, _i(1), _i(first), _stream(out))
+        # (that kernel multiplies the zero weights of hidden places with what pages hold there)
+        _call("attention_repair", "lsb_attention_repair", _p(qkv), _i(qkv.shape[1]), _p(cache.k_pages), _p(cache.v_pages),
+              *per_request, *sizes, _i(first), _i(0), _stream(out))
+        begin = end
+    if n_single or begin < end:
+        _call("attention", "lsb_paged_attention_generic_first", *common, _i(_dt(qkv)), _i(R), _i(ctx.max_q_len if begin < end else 1),
+              _i(n_single), _i(longest), _i(of_portions), *sizes, _f(softcap), _p(slopes), _i(first), _stream(out))
 
 
 # ----------------------------------------------- rows of a stream that is normed after the sum

@@ -39,6 +39,7 @@ SOURCES: Dict[str, object] = {          # library -> its source file (or files)
     "kv4_store": "kv4_store.cu",
     "attention_kv4": "attention_kv4.cu",
     "attention_kv4_f32": "attention_kv4_f32.cu",
+    "attention_repair": "attention_repair.cu",
     "gemm": "gemm.cu",
     "gemm_f32": "gemm_f32.cu",
     "gemm_tc": "gemm_tc.cu",

@@ -15,7 +15,7 @@ DTYPES = [torch.float32, torch.bfloat16]
 @pytest.fixture(scope="module")
 def ops():
     from llm_singularity_b200 import kernels
-    kernels.prepare(["kv4_store", "attention_kv4", "attention_kv4_f32"])
+    kernels.prepare(["kv4_store", "attention_kv4", "attention_kv4_f32", "attention_tc5", "attention_repair"])
     yield kernels
     kernels.check_status()
 
@@ -217,6 +217,23 @@ def test_single_tokens(ops, dtype, nh, nkv, hd):
 def test_portions(ops, dtype, nh, nkv, hd):
     _case(ops, dtype, nh, nkv, hd, [1, 2, 15, 40], [64, 2, 15, 81])
     _case(ops, dtype, nh, nkv, hd, [3, 1, 33], [300, 90, 120], window=20, first=4)
+
+
+@pytest.mark.parametrize("nh, nkv, hd", [(8, 2, 64), (4, 1, 128), (3, 3, 64)])
+def test_prompts_on_the_prompt_kernel(ops, nh, nkv, hd):
+    """Portions long enough to be expanded, beside single tokens and short portions, on every edge of its tiles."""
+    bf16 = torch.bfloat16
+    _case(ops, bf16, nh, nkv, hd, [128, 1, 200], [128, 70, 333])
+    _case(ops, bf16, nh, nkv, hd, [1, 257, 3], [9, 300, 64], page_size=32)
+    _case(ops, bf16, nh, nkv, hd, [130], [700], window=64, first=4)
+    _case(ops, bf16, nh, nkv, hd, [150, 300], [150, 900], window=100, first=70)
+    _case(ops, bf16, nh, nkv, hd, [129], [1000], window=1, first=1, page_size=64)
+    _case(ops, bf16, nh, nkv, hd, [140], [600], window=33, first=0)
+    _case(ops, bf16, nh, nkv, hd, [140], [600], window=300, first=1000)
+    _case(ops, bf16, nh, nkv, hd, [140], [600], window=40, first=4, fixed=True)
+    _case(ops, bf16, nh, nkv, hd, [150, 140], [200, 400], bad=[(0, 60), (1, 399)])
+    _case(ops, bf16, nh, nkv, hd, [150], [500], window=50, first=4, bad=[(0, 3), (0, 420)])
+    _case(ops, bf16, nh, nkv, hd, [150], [200], scale=-0.3)
 
 
 @pytest.mark.parametrize("window, first", [(1, 0), (1, 1), (1, 40), (16, 16), (17, 3), (64, 0), (64, 64), (200, 7), (5000, 4), (31, 1000)])
