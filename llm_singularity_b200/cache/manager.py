@@ -1,11 +1,12 @@
 """CacheManager: pages, block tables and state slots for every live request.
 
 Layers are sorted into groups by what their mixer needs: all past keys
-(``window is None``) or only the last ``window``.  Each group has its own
+(``window is None``), only the last ``window``, or those and the ``first`` few.  Each group has its own
 :class:`PagePool` and its own block table per request; a page id addresses one
 slot in the key pool and the value pool of every layer of the group.  Pages are
 taken before a step for the tokens that step brings, handed back when a request
-ends or, in a windowed group, as soon as the window has passed them, and reused.
+ends or, in a windowed group, as soon as the window has passed them (those of a request's
+first tokens stay if the group's layers see them), and reused.
 Mixers with per-request state of fixed size get one row per request slot
 instead of pages.  The slot of a request is also its row in the block tables.
 
@@ -35,9 +36,10 @@ class _Group:
     """One group's Python face: its pool and its host table are views into the memory layer."""
 
     def __init__(self, handle: _Handle, index: int, window: Optional[int], num_pages: int,
-                 slots: int, max_pages: int, page_size: int):
+                 slots: int, max_pages: int, page_size: int, first: Optional[int] = None):
         self.index = index
         self.window = window
+        self.first = first                             # tokens at a request's start that the window does not release (None: not said)
         self.page_size = page_size
         self.pool = PagePool(num_pages, _handle=handle, _group=index)
         self.cache_ids: List[int] = []
@@ -66,7 +68,7 @@ class CacheManager:
         self._store: Dict[int, object] = {}            # cache id -> what its spec allocated
         self._slots: Dict[Hashable, int] = {}          # request id -> slot
 
-        windows: List[Optional[int]] = []              # one entry per group, in order of first use
+        rules: List[Tuple[Optional[int], Optional[int]]] = []    # (window, first tokens) of each group, in order of first use
         members: List[List[int]] = []
         for cid, cs in enumerate(self._specs):
             if cs is None:
@@ -74,20 +76,23 @@ class CacheManager:
             if not isinstance(cs, CacheSpec):
                 raise TypeError(f"cache {cid}: {cs!r} is not a CacheSpec")
             if cs.paged:                               # caches with one release rule share a group
-                if cs.window not in windows:
-                    windows.append(cs.window)
+                rule = (cs.window, cs.first if cs.window is not None else None)
+                if rule not in rules:
+                    rules.append(rule)
                     members.append([])
-                g = windows.index(cs.window)
+                g = rules.index(rule)
                 members[g].append(cid)
                 self._group_of[cid] = g
-        sizes = [num_pages[w] if isinstance(num_pages, dict) else num_pages for w in windows]
+        sizes = [num_pages[w] if isinstance(num_pages, dict) else num_pages for w, _ in rules]
         if any(n <= 0 for n in sizes):
             raise ValueError(f"a page pool needs at least one page, got {sizes}")
         self._h = _Handle(page_size, max_requests, max_pages_per_request,
-                          [-1 if w is None else w for w in windows], sizes)
+                          [-1 if w is None else w for w, _ in rules], sizes)
         self._lib, self._ptr = self._h.lib, self._h.ptr
-        for g, (w, n) in enumerate(zip(windows, sizes)):
-            grp = _Group(self._h, g, w, n, max_requests, max_pages_per_request, page_size)
+        for g, ((w, first), n) in enumerate(zip(rules, sizes)):
+            if first is not None and self._lib.lsbm_keep_first(self._ptr, g, first) == native.ERR:
+                raise self._fail()
+            grp = _Group(self._h, g, w, n, max_requests, max_pages_per_request, page_size, first)
             grp.cache_ids = members[g]
             self.groups.append(grp)
         self._page_buf = (ctypes.c_int * max_pages_per_request)()

@@ -21,6 +21,7 @@ _IP = POINTER(c_int)
 _SIGNATURES = {
     "lsbm_create": (c_void_p, [c_int, c_int, c_int, c_int, _IP, _IP]),
     "lsbm_destroy": (None, [c_void_p]),
+    "lsbm_keep_first": (c_int, [c_void_p, c_int, c_longlong]),
     "lsbm_last_error": (c_char_p, [c_void_p]),
     "lsbm_pool_allocate": (c_int, [c_void_p, c_int]),
     "lsbm_pool_retain": (c_int, [c_void_p, c_int, c_int]),

@@ -42,6 +42,11 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--max-tokens-per-batch", type=int, default=2048)
     ap.add_argument("--prefill-chunk", type=int, default=None)
     ap.add_argument("--no-prefix-cache", action="store_true")
+    ap.add_argument("--kv-cache", choices=["compute", "int4"], default="compute",
+                    help="keys and values in the compute dtype, or in 4 bits with a scale for every 32 dims")
+    ap.add_argument("--window", type=int, default=None,
+                    help="let every token see the last so many only (pages behind the window go back)")
+    ap.add_argument("--first-tokens", type=int, default=0, help="... and the first so many of its sequence")
     ap.add_argument("--prompt-ids", help="file with prompts as token ids")
     ap.add_argument("--prompt-len", type=int, default=16)
     ap.add_argument("--num-requests", type=int, default=1)
@@ -137,7 +142,8 @@ def main(argv=None) -> int:
                  dtype=args.dtype, device=args.device, kv_block_size=args.kv_block_size,
                  num_kv_blocks=args.num_kv_blocks, max_batch_size=args.max_batch_size,
                  max_tokens_per_batch=args.max_tokens_per_batch, prefill_chunk=args.prefill_chunk,
-                 prefix_cache=not args.no_prefix_cache, verbose=True)
+                 prefix_cache=not args.no_prefix_cache, verbose=True, kv_cache=args.kv_cache,
+                 window=args.window, first_tokens=args.first_tokens)
     if args.bench:
         print(json.dumps(run_bench(eng, args)))
         return 0

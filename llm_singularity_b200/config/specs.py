@@ -13,7 +13,7 @@ what replaces the ``-DMODEL=llama`` compile-time switch (CMakeLists.txt:12,27).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Optional, Tuple
 
 
@@ -89,7 +89,9 @@ class NoPositionSpec(PartSpec):
 # --------------------------------------------------------------------------- mixers
 @dataclass(frozen=True)
 class AttentionSpec(PartSpec):
-    """Causal softmax attention with grouped keys/values over a paged cache."""
+    """Causal softmax attention with grouped keys/values over a paged cache.  ``first_tokens``: with a window, the
+    first so many tokens of a sequence stay visible.  ``cache_bits`` 4: keys and values are cached in 4 bits with a
+    scale for every 32 dims of a head (None: in the compute dtype)."""
 
     hidden_size: int = 0
     num_heads: int = 0
@@ -102,6 +104,8 @@ class AttentionSpec(PartSpec):
     # a linear position bias -slope[h] * distance with the usual geometric slopes over the heads
     logit_softcap: Optional[float] = None
     linear_bias: bool = False
+    first_tokens: Optional[int] = None    # (where it is said, a sequence may outgrow the pool: ``CacheSpec.first``)
+    cache_bits: Optional[int] = None
     kind: str = field(init=False, default="attention")
 
 
@@ -563,3 +567,29 @@ class ModelSpec:
     @property
     def num_caches(self) -> int:
         return 1 + max((c.cache for c in self.order), default=-1)
+
+
+# ----------------------------------------------------------------- long contexts
+KV_CACHES = {"compute": None, "int4": 4}          # how keys and values may be cached: their bits (None: the compute dtype)
+
+
+def with_long_context(spec: ModelSpec, kv_cache: str = "compute", window: Optional[int] = None, first_tokens: int = 0) -> ModelSpec:
+    """``spec`` as it is served with other caches: keys and values held as ``kv_cache`` says, and, with a ``window``, every
+    query seeing the last ``window`` tokens and the first ``first_tokens`` only, so that a sequence may grow without end in
+    bounded memory.  For models whose layers all mix by ``AttentionSpec``; others have caches of their own."""
+    if kv_cache not in KV_CACHES:
+        raise ValueError(f"kv_cache must be one of {sorted(KV_CACHES)}, got {kv_cache!r}")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if first_tokens < 0 or (first_tokens and window is None):
+        raise ValueError(f"first_tokens {first_tokens} must not be negative, and goes with a window")
+    if kv_cache == "compute" and window is None:
+        return spec
+    other = next((b.mixer.kind for b in spec.blocks if not isinstance(getattr(b, "mixer", None), AttentionSpec)), None)
+    if other is not None:
+        raise ValueError(f"{spec.architecture}: 4-bit caches and windows can be asked for where every layer is plain "
+                         f"attention; this model has '{other}'")
+    change = dict(cache_bits=KV_CACHES[kv_cache])
+    if window is not None:
+        change.update(window=window, first_tokens=first_tokens)
+    return replace(spec, blocks=tuple(replace(b, mixer=replace(b.mixer, **change)) for b in spec.blocks))

@@ -39,9 +39,11 @@ struct Pool {
 
 struct Group {
     int window = -1;                 // < 0: the group keeps all keys
+    int kept = -1;                   // pages at a request's start that no window releases; < 0: none, and the group's
+                                     // requests are taken to need all of their pages at once
     Pool pool;
     std::vector<int32_t> table;      // [slots * max_pages], host mirror of the device table
-    std::vector<int32_t> first_live; // per slot: pages [0, first_live) were released behind the window
+    std::vector<int32_t> first_live; // per slot: pages [kept, first_live) were released behind the window
     std::vector<int32_t> updates;    // (flat index, value) pairs not yet taken
     std::vector<uint32_t> taken;     // per cell: the call of take_updates_last that last gave it out
     uint32_t take_call = 0;
@@ -172,14 +174,49 @@ LSB_API void* lsbm_create(int page_size, int max_requests, int max_pages, int n_
 
 LSB_API void lsbm_destroy(void* h) { delete M(h); }
 
+// Pages that hold a request's first `tokens` positions stay in group g until the request is closed, however far its window has
+// passed.  Before the first request is opened.
+LSB_API int lsbm_keep_first(void* h, int g, long long tokens) {
+    Memory* m = M(h);
+    if (no_group(m, g)) return kErr;
+    if (tokens < 0) return m->fail("a group cannot keep fewer than no tokens");
+    if ((int)m->free_slots.size() != m->max_requests) return m->fail("what a group keeps is said before a request is open");
+    m->groups[g].kept = (int)std::min<long long>(m->pages_for(tokens), m->max_pages);
+    return 0;
+}
+
 LSB_API const char* lsbm_last_error(void* h) { return M(h)->error.c_str(); }
 LSB_API int lsbm_page_size(void* h) { return M(h)->page_size; }
 LSB_API int lsbm_max_pages(void* h) { return M(h)->max_pages; }
-// Pages of the smallest pool (1 << 30 if there is none): what a single request can ever hold.
-LSB_API int lsbm_smallest_pool(void* h) {
-    int n = 1 << 30;
-    for (Group& g : M(h)->groups) n = std::min(n, g.pool.num_pages);
-    return n;
+// Pages of group g that a request of `tokens` tokens cannot do without at once.  Behind a window pages go back step by step, so
+// where the group says what it keeps they are the first tokens', the window's (which may begin inside a page) and one for a
+// step's; else all that the tokens fill.
+static long long least_pages(Memory* m, const Group& g, long long tokens) {
+    const long long all = m->pages_for(tokens);
+    return g.window >= 0 && g.kept >= 0 ? std::min(all, g.kept + m->pages_for(g.window) + 2) : all;
+}
+// The same of the group whose pool has the least beyond them; *pool is that pool's size.
+LSB_API long long lsbm_least_pages(void* h, long long tokens, int* pool) {
+    Memory* m = M(h);
+    long long least = m->pages_for(tokens);
+    *pool = 1 << 30;
+    bool any = false;
+    for (const Group& g : m->groups) {
+        const long long need = least_pages(m, g, tokens);
+        if (!any || g.pool.num_pages - need < *pool - least) {
+            least = need;
+            *pool = g.pool.num_pages;
+        }
+        any = true;
+    }
+    return least;
+}
+// Whether every group has them free for a request that has `had` of its pages already and may count on `more` beyond the free ones.
+LSB_API int lsbm_has_room(void* h, long long tokens, int had, int more) {
+    Memory* m = M(h);
+    for (const Group& g : m->groups)
+        if (least_pages(m, g, tokens) - had > (long long)g.pool.free_list.size() + more) return 0;
+    return 1;
 }
 
 // ----------------------------------------------------------------------------- pools
@@ -279,7 +316,7 @@ LSB_API int lsbm_commit(void* h, int slot, long long new_length) {
         // the next query sits at position >= new_length and sees keys > position - window
         const long long first_needed = std::max(0LL, new_length - g.window + 1);
         const int dead = (int)std::min<long long>(first_needed / m->page_size, r->num_pages);
-        for (int i = g.first_live[slot]; i < dead; ++i) {
+        for (int i = std::max(g.first_live[slot], g.kept); i < dead; ++i) {
             if (m->pool_release((int)gi, g.table[(size_t)slot * m->max_pages + i]) == kErr) return kErr;
             m->set_cell(g, slot, i, kNoPage);
         }
@@ -295,7 +332,8 @@ LSB_API int lsbm_close(void* h, int slot) {
     if (!r) return kErr;
     for (size_t gi = 0; gi < m->groups.size(); ++gi) {
         Group& g = m->groups[gi];
-        for (int i = g.first_live[slot]; i < r->num_pages; ++i) {
+        for (int i = 0; i < r->num_pages; ++i) {
+            if (i >= g.kept && i < g.first_live[slot]) continue;       // released behind the window
             if (m->pool_release((int)gi, g.table[(size_t)slot * m->max_pages + i]) == kErr) return kErr;
             m->set_cell(g, slot, i, kNoPage);
         }
@@ -638,7 +676,7 @@ LSB_API int lsbm_check(void* h) {
             const int covered = r.open ? r.num_pages : 0;
             for (int i = 0; i < covered; ++i) {
                 const int p = row[i];
-                if (i < g.first_live[slot]) {
+                if (i >= g.kept && i < g.first_live[slot]) {
                     if (p != kNoPage) return m->fail("released cell still names page " + std::to_string(p));
                     continue;
                 }

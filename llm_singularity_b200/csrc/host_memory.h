@@ -9,7 +9,8 @@ extern "C" {
 const char* lsbm_last_error(void* h);
 int lsbm_page_size(void* h);
 int lsbm_max_pages(void* h);
-int lsbm_smallest_pool(void* h);
+long long lsbm_least_pages(void* h, long long tokens, int* pool);
+int lsbm_has_room(void* h, long long tokens, int had, int more);
 int lsbm_open(void* h);
 int lsbm_close(void* h, int slot);
 long long lsbm_length(void* h, int slot);

@@ -161,11 +161,12 @@ void fail_request(Scheduler* s, int id, const std::string& why) {
 // Why the request can never run (its tokens plus one exceed the model's length or the pool), or "".
 std::string never_fits(Scheduler* s, const Req& r) {
     const long long have = (long long)r.tokens.size(), n = have + 1;
-    const long long pool = lsbm_smallest_pool(s->mem);
+    int pool = 0;
+    const long long least = lsbm_least_pages(s->mem, n, &pool);
     if (n > s->max_model_len)
         return std::to_string(have) + " tokens plus one exceed max_model_len " + std::to_string(s->max_model_len);
-    if (s->pages_for(n) > std::min<long long>(pool, lsbm_max_pages(s->mem)))
-        return std::to_string(have) + " tokens plus one need " + std::to_string(s->pages_for(n)) +
+    if (least > pool || s->pages_for(n) > lsbm_max_pages(s->mem))
+        return std::to_string(have) + " tokens plus one need " + std::to_string(least > pool ? least : s->pages_for(n)) +
                " pages, the pool has " + std::to_string(pool);
     return "";
 }
@@ -262,14 +263,13 @@ int plan(Scheduler* s, bool ahead) {
                                 (int)s->scratch_nodes.size());
             if (n_path == kErr) return s->mem_fail();
         }
-        const long long need = s->pages_for((long long)r.tokens.size() + 1) - n_path;
         // pages on the matched path are in use by this request, not evictable for it
         int idle_on_path = 0;
         if (n_path > 0) {
             idle_on_path = lsbp_idle_on(s->mem, s->scratch_nodes.data(), n_path);
             if (idle_on_path == kErr) return s->mem_fail();
         }
-        if (need > s->free_pages() - idle_on_path) break;
+        if (!lsbm_has_room(s->mem, (long long)r.tokens.size() + 1, n_path, (s->prefix ? lsbp_evictable(s->mem) : 0) - idle_on_path)) break;
         const int slot = lsbm_open(s->mem);
         if (slot < 0) break;
         s->waiting.pop_front();

@@ -41,9 +41,11 @@ class Engine:
                  num_kv_blocks: int = 1024, max_batch_size: int = 64,
                  max_tokens_per_batch: int = 2048, prefill_chunk: Optional[int] = None,
                  max_model_len: Optional[int] = None, prefix_cache: bool = True,
-                 config=None, ops=None, verbose: bool = False, run_ahead: bool = True):
+                 config=None, ops=None, verbose: bool = False, run_ahead: bool = True, kv_cache: str = "compute",
+                 window: Optional[int] = None, first_tokens: int = 0):
         """``model_dir`` holds config.json and, unless ``random_weights``, the safetensors
-        files.  Defaults follow the reference's hints: pages of 16 tokens, 1024 pages, 2048
+        files.  ``kv_cache``, ``window`` and ``first_tokens`` are those of :class:`ModelRunner`: keys and values in 4
+        bits ("int4"), and a sliding window beside the first tokens.  Defaults follow the reference's hints: pages of 16 tokens, 1024 pages, 2048
         tokens per batch (models/llama/llama_model.cpp:111-120)."""
         tensors = None
         if random_weights:
@@ -59,7 +61,8 @@ class Engine:
                                   device=device, page_size=kv_block_size, num_pages=num_kv_blocks,
                                   max_requests=max_batch_size,
                                   max_tokens_per_step=max_tokens_per_batch,
-                                  max_model_len=max_model_len, ops=ops, verbose=verbose)
+                                  max_model_len=max_model_len, ops=ops, verbose=verbose, kv_cache=kv_cache,
+                                  window=window, first_tokens=first_tokens)
         cache = self.runner.cache
         shareable = prefix_cache and cache.groups and all(g.window is None for g in cache.groups) \
             and all(s is not None and s.shareable for s in self.runner.model.cache_specs())

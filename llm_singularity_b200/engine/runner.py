@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheManager
-from ..config.specs import ModelSpec
+from ..config.specs import ModelSpec, with_long_context
 from ..models.decoder import DecoderModel
 from ..parts.base import Runtime
 from ..registry import architecture_of, config_of, read_config_json
@@ -98,9 +98,15 @@ class ModelRunner:
                  dtype="bfloat16", device="cuda:0", page_size: int = 16,
                  num_pages: int = 1024, max_requests: int = 64,
                  max_tokens_per_step: int = 2048, max_model_len: Optional[int] = None,
-                 ops=None, verbose: bool = False, cuda_graphs: bool = True):
+                 ops=None, verbose: bool = False, cuda_graphs: bool = True, kv_cache: str = "compute",
+                 window: Optional[int] = None, first_tokens: int = 0):
         """Either ``model_dir`` (config.json + safetensors) or ``config`` + ``tensors``
-        (checkpoint names -> tensors, e.g. from ``random_tensors``)."""
+        (checkpoint names -> tensors, e.g. from ``random_tensors``).
+
+        ``kv_cache`` "int4" holds keys and values in 4 bits (``page_size`` a multiple of 16, heads of a
+        multiple of 32); ``window`` lets every token see the last so many and the first
+        ``first_tokens`` of its sequence only, and the pages between go back to the pool
+        (``config.specs.with_long_context`` says for which models)."""
         self.dtype = parse_dtype(dtype)
         arch = None
         if config is None:
@@ -108,7 +114,7 @@ class ModelRunner:
             arch = architecture_of(cfg_dict)
             config = config_of(model_dir, cfg_dict)
         self.config = config
-        self.spec: ModelSpec = config.to_model_spec()
+        self.spec: ModelSpec = with_long_context(config.to_model_spec(), kv_cache, window, first_tokens)
         self.rt = Runtime(device, self.dtype, ops=ops, page_size=page_size)
         self.model = _build_model(self.spec, self.rt, arch)
         if ops is None:

@@ -71,11 +71,15 @@ class CacheSpec:
     ``bytes_per_page(page_size, element_size)`` -> bytes one page id stands for in this cache.
     ``shareable``: full pages of this kind mean the same for every request with the same
     tokens before them, so a prefix tree may hand them to other requests.
+    ``first``: of a windowed kind, how many tokens at a request's start the window leaves alone; kinds
+    share a group if this is the same too.  Where it is said (0 too) a request counts in its group for the pages
+    of its first tokens, its window and a step, so a sequence may be longer than the pool; None: for all of its pages.
     """
 
     paged = False
     shareable = False
     window: Optional[int] = None
+    first: Optional[int] = None
 
     def allocate(self, rt, page_size: int, num_pages: Optional[int], slots: int):
         raise NotImplementedError
@@ -117,6 +121,7 @@ class PagedKVSpec(CacheSpec):
     head_dim: int
     window: Optional[int] = None
     value_dim: Optional[int] = None        # size of a value where it is not the keys' (None: head_dim)
+    first: Optional[int] = None            # ... and of the first so many, with a window
     paged = True
     shareable = True
 
@@ -144,6 +149,34 @@ class KV4CacheView:
     page_size: int
     window: Optional[int]
     group: int
+
+
+@dataclass(frozen=True)
+class PagedKV4Spec(CacheSpec):
+    """Keys and values in 4 bits with a scale for every 32 dims of a head (``csrc/kv4.cuh``): 9/32 of
+    the bytes of bfloat16, whatever the compute dtype."""
+
+    num_kv_heads: int
+    head_dim: int
+    window: Optional[int] = None
+    first: Optional[int] = None
+    paged = True
+    shareable = True
+
+    def __post_init__(self):
+        if self.head_dim % 32 or not 32 <= self.head_dim <= 256:
+            raise ValueError(f"a 4-bit cache holds heads of a multiple of 32 up to 256, got {self.head_dim}")
+
+    def allocate(self, rt, page_size, num_pages, slots):
+        if page_size % 16:
+            raise ValueError(f"a 4-bit cache has pages of a multiple of 16 tokens, got {page_size}")
+        return torch.zeros((num_pages, self.num_kv_heads, page_size // 16, 18 * self.head_dim), dtype=torch.uint8, device=rt.device)
+
+    def view(self, storage, group):
+        return KV4CacheView(storage, group.dev_table, group.page_size, group.window, group.index)
+
+    def bytes_per_page(self, page_size, element_size):
+        return self.num_kv_heads * page_size * 18 * self.head_dim // 16
 
 
 @dataclass
@@ -217,6 +250,8 @@ class CompositeCacheSpec(CacheSpec):
         windows = {p.window for p in self.parts if p.paged}
         if len(windows) > 1:
             raise ValueError(f"the paged parts of one cache must share a window, got {sorted(map(str, windows))}")
+        if len({p.first for p in self.parts if p.paged}) > 1:
+            raise ValueError("the paged parts of one cache must leave the same first tokens alone")
 
     @property
     def paged(self):
@@ -225,6 +260,10 @@ class CompositeCacheSpec(CacheSpec):
     @property
     def window(self):
         return next((p.window for p in self.parts if p.paged), None)
+
+    @property
+    def first(self):
+        return next((p.first for p in self.parts if p.paged), None)
 
     @property
     def shareable(self):
