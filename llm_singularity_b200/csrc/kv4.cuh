@@ -39,13 +39,17 @@ __device__ __forceinline__ float kv4_scale(float largest) {
     return __uint_as_float((bits + 0x3ffffu + (bits >> 19 & 1u)) & ~0x7ffffu);
 }
 
-// The whole number in [-7, 7] nearest to x / s, ties to even.  The quotient in 32-bit may round onto a border between two
-// numbers or across it; what is left of x after k steps of s is exact in sign (k s has 8 bits), and settles it.
-__device__ __forceinline__ int kv4_code(float x, float s) {
-    if (s == 0.f) return 0;
-    float k = rintf(__fdiv_rn(x, s));
-    const float left = fmaf(-k, s, x), half = 0.5f * s;
-    if (left > half || (left == half && ((int)k & 1))) k += 1.f;
-    else if (left < -half || (left == -half && ((int)k & 1))) k -= 1.f;
-    return max(-7, min(7, (int)k));
+// The whole number nearest to x / s, ties to even, plus 8; |x| is at most the group's largest magnitude (of which s is a seventh but
+// for 1/32, so the number is from -7 to 7), and 0 where s is; `inverse` is about 1 / s.  The product in 32-bit may fall on the
+// other side of a border between two numbers; what is left of x after k steps of s is exact in sign (k s has 8 bits), and settles it: a
+// step more where it is above half of one, or is half and the number odd.  Adding 1.5 * 2^23 rounds to a whole number and leaves it in
+// the low bits; magnitudes compare as their bits do.
+__device__ __forceinline__ uint32_t kv4_code(float x, float s, float inverse) {
+    constexpr float kWhole = 12582912.f;
+    constexpr uint32_t kWholeBits = 0x4b400000u;
+    const float t = fmaf(x, inverse, kWhole), left = fmaf(kWhole - t, s, x);
+    uint32_t n = __float_as_uint(t);
+    const uint32_t off = __float_as_uint(left) & 0x7fffffffu, half = __float_as_uint(0.5f * s);
+    if (off + (n & 1u) > half) n += (uint32_t)(__float_as_int(left) >> 31 | 1);
+    return n - (kWholeBits - 8u);
 }

@@ -50,128 +50,143 @@ template <> struct Four<__nv_bfloat16> {
     }
 };
 
+// One element of a head at x, rotated in 64-bit by the token's angles and rounded to the type.
 template <typename T>
+__device__ __forceinline__ float turned(const T* x, int d, int half, const double (*cs)[kMaxDim / 2]) {
+    if (d >= 2 * half) return lsb_to_float(x[d]);
+    const bool low = d < half;
+    const int i = low ? d : d - half;
+    const double own = (double)lsb_to_float(x[d]), other = (double)lsb_to_float(x[low ? d + half : i]);
+    return lsb_to_float(lsb_from_float<T>((float)(other * (low ? -cs[1][i] : cs[1][i]) + own * cs[0][i])));
+}
+
+// A lane takes four dims of the token's keys and values, as they stand side by side in the projection, eight lanes a group; its
+// codes are half a word of a key's row, or two bytes of a value's, which meet their neighbours' by a shuffle.
+template <int G, typename T>
 __global__ void __launch_bounds__(kStoreThreads) rope_kv4_store_kernel(const StoreParams p) {
-    __shared__ double cs64[2][kMaxDim / 2];
-    __shared__ float cs[2][kMaxDim / 2];
-    __shared__ __align__(16) unsigned char rows[kStoreThreads / 32][kMaxDim / 2];
+    constexpr int HD = kKv4Group * G, TILE = kv4_tile_bytes(HD);
+    __shared__ __align__(16) double cs64[2][kMaxDim / 2];
+    __shared__ __align__(16) float cs[2][kMaxDim / 2];
+    __shared__ long long place;                                 // tile of the token in the pool's first head, -1 for none
+    __shared__ int offset;                                      // its row there
     lsb_pdl_launch_dependents();
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int hd = p.hd, half = p.rotary_dim >> 1;
+    const int half = p.rotary_dim >> 1;
     // (positions are metadata of the step, on the device before its first kernel: the angles need not wait for the projection)
     const int pos = p.positions[t];
     for (int i = tid; i < half; i += kStoreThreads) {
-        sincos((double)pos * (double)p.inv_freq[i], &cs64[1][i], &cs64[0][i]);
-        cs[0][i] = (float)cs64[0][i];
-        cs[1][i] = (float)cs64[1][i];
+        double sine, cosine;
+        sincos((double)pos * (double)p.inv_freq[i], &sine, &cosine);
+        cs64[0][i] = cosine;
+        cs64[1][i] = sine;
+        cs[0][i] = (float)cosine;
+        cs[1][i] = (float)sine;
+    }
+    lsb_pdl_wait();
+    if (tid == kStoreThreads - 1) {                             // (of the warp that has the fewest angles)
+        const int pi = pos / p.page_size, within = pos - pi * p.page_size;
+        int page = -1;
+        if (p.store && pi < p.table_stride) page = p.block_table[(size_t)p.table_rows[p.token_req[t]] * p.table_stride + pi];
+        const bool held = page >= 0 && page < p.num_pages;
+        if (p.store && !held) lsb_set_status(LSB_BAD_PAGE);
+        place = held ? (long long)page * p.nkv * (p.page_size / kKv4Tile) + within / kKv4Tile : -1;
+        offset = within % kKv4Tile;
     }
     __syncthreads();
-    lsb_pdl_wait();
-    const T* row = reinterpret_cast<const T*>(p.qkv) + (size_t)t * (p.nh + 2 * p.nkv) * hd;
-    T* q = reinterpret_cast<T*>(p.q_out) + (size_t)t * p.nh * hd;
+    const T* row = reinterpret_cast<const T*>(p.qkv) + (size_t)t * (p.nh + 2 * p.nkv) * HD;
+    T* q = reinterpret_cast<T*>(p.q_out) + (size_t)t * p.nh * HD;
 
     if (p.vec) {
-        const int quads = half >> 2, per = (hd >> 2) - quads;              // per head: fours of pairs, then the fours that pass
-        for (int idx = tid; idx < p.nh * per; idx += kStoreThreads) {
-            const int h = idx / per, c = idx - h * per;
+        const int quads = half >> 2, per = HD / 4 - quads;                 // per head: fours of pairs, then the fours that pass
+        const int step_h = kStoreThreads / per, step_c = kStoreThreads - step_h * per;
+        for (int h = tid / per, c = tid - h * per; h < p.nh; h += step_h, c += step_c) {
+            if (c >= per) { c -= per; if (++h >= p.nh) break; }
+            const T* from = row + h * HD;
+            T* to = q + h * HD;
             float a[4], b[4];
             if (c < quads) {
                 const int i = 4 * c;
-                Four<T>::load(row + h * hd + i, a);
-                Four<T>::load(row + h * hd + half + i, b);
+                Four<T>::load(from + i, a);
+                Four<T>::load(from + half + i, b);
+                const float4 cosine = *reinterpret_cast<const float4*>(&cs[0][i]), sine = *reinterpret_cast<const float4*>(&cs[1][i]);
+                const float c4[4] = {cosine.x, cosine.y, cosine.z, cosine.w}, s4[4] = {sine.x, sine.y, sine.z, sine.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float x0 = a[e], x1 = b[e];
-                    a[e] = x0 * cs[0][i + e] - x1 * cs[1][i + e];
-                    b[e] = x0 * cs[1][i + e] + x1 * cs[0][i + e];
+                    a[e] = x0 * c4[e] - x1 * s4[e];
+                    b[e] = x0 * s4[e] + x1 * c4[e];
                 }
-                Four<T>::store(q + h * hd + i, a);
-                Four<T>::store(q + h * hd + half + i, b);
+                Four<T>::store(to + i, a);
+                Four<T>::store(to + half + i, b);
             } else {
-                const int i = 4 * (c + quads);
-                Four<T>::load(row + h * hd + i, a);
-                Four<T>::store(q + h * hd + i, a);
+                Four<T>::load(from + 4 * (c + quads), a);
+                Four<T>::store(to + 4 * (c + quads), a);
             }
         }
     } else {
-        const int per = hd - half;
+        const int per = HD - half;
         for (int idx = tid; idx < p.nh * per; idx += kStoreThreads) {
             const int h = idx / per, c = idx - h * per;
             if (c < half) {
-                const float x0 = lsb_to_float(row[h * hd + c]), x1 = lsb_to_float(row[h * hd + half + c]);
-                q[h * hd + c] = lsb_from_float<T>(x0 * cs[0][c] - x1 * cs[1][c]);
-                q[h * hd + half + c] = lsb_from_float<T>(x0 * cs[1][c] + x1 * cs[0][c]);
+                const float x0 = lsb_to_float(row[h * HD + c]), x1 = lsb_to_float(row[h * HD + half + c]);
+                q[h * HD + c] = lsb_from_float<T>(x0 * cs[0][c] - x1 * cs[1][c]);
+                q[h * HD + half + c] = lsb_from_float<T>(x0 * cs[1][c] + x1 * cs[0][c]);
             } else {
-                q[h * hd + half + c] = row[h * hd + half + c];
+                q[h * HD + half + c] = row[h * HD + half + c];
             }
         }
     }
-    if (!p.store) return;
+    if (place < 0) return;
 
-    int page = -1;
-    if (pos / p.page_size < p.table_stride)
-        page = p.block_table[(size_t)p.table_rows[p.token_req[t]] * p.table_stride + pos / p.page_size];
-    if (page < 0 || page >= p.num_pages) {
-        if (tid == 0) lsb_set_status(LSB_BAD_PAGE);
-        return;
-    }
-    const int G = hd / kKv4Group, within = pos % p.page_size, r = within % kKv4Tile;
-    for (int item = warp; item < 2 * p.nkv; item += kStoreThreads / 32) {
-        const bool value = item >= p.nkv;
-        const int h = value ? item - p.nkv : item;
-        unsigned char* tile = p.pages + (((size_t)page * p.nkv + h) * (p.page_size / kKv4Tile) + within / kKv4Tile) * kv4_tile_bytes(hd);
-        const T* x = row + (size_t)(p.nh + item) * hd;
-        for (int base = 0; base < hd; base += 128) {            // four dims a lane, a group to eight lanes
-            const int d0 = base + 4 * lane;
-            float y[4] = {0.f, 0.f, 0.f, 0.f};
-            if (d0 < hd) {
+    const int r = offset, o = lane & 7, tiles = p.page_size / kKv4Tile, n = 2 * p.nkv * HD;
+    unsigned char* tile0 = p.pages + place * TILE;
+    for (int base = warp * 128; base < n; base += kStoreThreads * 4) {
+        const int f = base + 4 * lane, item = f / HD, d0 = f - item * HD, g = d0 / kKv4Group;
+        const bool there = f < n, value = item >= p.nkv;
+        const T* x = row + (size_t)(p.nh + item) * HD;
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        if (there && p.vec) {                                   // the four are of a pair's first dims, of its second ones or of none
+            Four<T>::load(x + d0, y);
+            if (!value && d0 < 2 * half) {
+                const bool low = d0 < half;
+                const int i = low ? d0 : d0 - half;
+                float other[4];
+                Four<T>::load(x + (low ? d0 + half : i), other);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int d = d0 + e;
-                    y[e] = lsb_to_float(x[d]);
-                    if (!value && d < 2 * half) {
-                        const int i = d < half ? d : d - half;
-                        const double x0 = d < half ? (double)y[e] : (double)lsb_to_float(x[i]);
-                        const double x1 = d < half ? (double)lsb_to_float(x[i + half]) : (double)y[e];
-                        const double z = d < half ? x0 * cs64[0][i] - x1 * cs64[1][i] : x0 * cs64[1][i] + x1 * cs64[0][i];
-                        y[e] = lsb_to_float(lsb_from_float<T>((float)z));
-                    }
+                    const double sine = low ? -cs64[1][i + e] : cs64[1][i + e];
+                    y[e] = lsb_to_float(lsb_from_float<T>((float)((double)other[e] * sine + (double)y[e] * cs64[0][i + e])));
                 }
             }
-            float top = 0.f;
-            bool fine = true;
+        } else if (there) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                fine = fine && fabsf(y[e]) <= FLT_MAX;
-                top = fmaxf(top, fabsf(y[e]));
-            }
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            fine = (__ballot_sync(0xffffffffu, fine) >> (lane & 24) & 0xffu) == 0xffu;
-            const float s = fine ? kv4_scale(top) : 0.f;
-            uint32_t code = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) code |= (uint32_t)(kv4_code(y[e], s) + 8) << (4 * e);
-            if (d0 < hd) {
-                const int g = d0 / kKv4Group, o = lane & 7;
-                if (value) {
-                    const int i = 2 * g + (o >> 2), e = 2 * (o & 3);
-                    rows[warp][e * 2 * G + i] = (unsigned char)(code & 0xffu);
-                    rows[warp][(e + 1) * 2 * G + i] = (unsigned char)(code >> 8);
-                } else {
-                    *reinterpret_cast<unsigned short*>(&rows[warp][((o >> 1) * G + g) * 4 + (o & 1) * 2]) = (unsigned short)code;
-                }
-                if (o == 0) {
-                    const int at = (value ? kv4_value_scales_at(hd) : kv4_key_scales_at(hd)) + (r * G + g) * 2;
-                    *reinterpret_cast<__nv_bfloat16*>(tile + at) =
-                        fine ? __float2bfloat16_rn(s) : __ushort_as_bfloat16((unsigned short)0x7fff);
-                }
-            }
+            for (int e = 0; e < 4; ++e) y[e] = value ? lsb_to_float(x[d0 + e]) : turned(x, d0 + e, half, cs64);
         }
-        __syncwarp();
-        uint32_t* to = reinterpret_cast<uint32_t*>(tile + (value ? kv4_values_at(hd) : 0) + r * (hd / 2));
-        for (int w = lane; w < hd / 8; w += 32) to[w] = reinterpret_cast<const uint32_t*>(rows[warp])[w];
-        __syncwarp();
+        float zero = 0.f;                                       // times a number 0, times anything else NaN
+#pragma unroll
+        for (int e = 0; e < 4; ++e) zero = fmaf(y[e], 0.f, zero);
+        bool fine = zero == 0.f;
+        float top = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        fine = (__ballot_sync(0xffffffffu, fine) >> (lane & 24) & 0xffu) == 0xffu;
+        const float s = fine ? kv4_scale(top) : 0.f, inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
+        uint32_t code = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) code |= kv4_code(s > 0.f ? y[e] : 0.f, s, inverse) << (4 * e);
+        const uint32_t pair = __shfl_xor_sync(0xffffffffu, code, 1), across = __shfl_xor_sync(0xffffffffu, code, 4);
+        if (!there) continue;
+        unsigned char* tile = tile0 + (size_t)(value ? item - p.nkv : item) * tiles * TILE;
+        if (value) {                                            // dims 16 i + 2 e and + 1: i = 2 g + o / 4, e = 2 (o % 4) and + 1
+            const bool front = o < 4;
+            const uint32_t two = front ? (code & 0xffu) | (across & 0xffu) << 8 : (across >> 8 & 0xffu) | (code >> 8 & 0xffu) << 8;
+            *reinterpret_cast<unsigned short*>(tile + kv4_values_at(HD) + r * (HD / 2) + (2 * (o & 3) + (front ? 0 : 1)) * 2 * G + 2 * g) = (unsigned short)two;
+        } else if (!(o & 1)) {                                  // dims 8 t .. 8 t + 7 of the group: t = o / 2
+            *reinterpret_cast<uint32_t*>(tile + r * (HD / 2) + ((o >> 1) * G + g) * 4) = code | pair << 16;
+        }
+        if (o == 0)
+            *reinterpret_cast<__nv_bfloat16*>(tile + (value ? kv4_value_scales_at(HD) : kv4_key_scales_at(HD)) + (r * G + g) * 2) =
+                fine ? __float2bfloat16_rn(s) : __ushort_as_bfloat16((unsigned short)0x7fff);
     }
 }
 
@@ -303,7 +318,20 @@ LSB_API int lsb_rope_kv4_store(const void* qkv, int dtype, int n_tokens, int nh,
     p.table_stride = table_stride; p.pages = (unsigned char*)pages;
     p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.num_pages = num_pages; p.store = store;
     p.vec = rotary_dim % 8 == 0 && (uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0;
-    LSB_DISPATCH_DTYPE(dtype, return lsb_launch(rope_kv4_store_kernel<T>, dim3(n_tokens), dim3(kStoreThreads), 0, stream, 1, p));
+    const dim3 grid(n_tokens), block(kStoreThreads);
+    LSB_DISPATCH_DTYPE(dtype, {
+        switch (hd) {
+            case 32: return lsb_launch(rope_kv4_store_kernel<1, T>, grid, block, 0, stream, 1, p);
+            case 64: return lsb_launch(rope_kv4_store_kernel<2, T>, grid, block, 0, stream, 1, p);
+            case 96: return lsb_launch(rope_kv4_store_kernel<3, T>, grid, block, 0, stream, 1, p);
+            case 128: return lsb_launch(rope_kv4_store_kernel<4, T>, grid, block, 0, stream, 1, p);
+            case 160: return lsb_launch(rope_kv4_store_kernel<5, T>, grid, block, 0, stream, 1, p);
+            case 192: return lsb_launch(rope_kv4_store_kernel<6, T>, grid, block, 0, stream, 1, p);
+            case 224: return lsb_launch(rope_kv4_store_kernel<7, T>, grid, block, 0, stream, 1, p);
+            case 256: return lsb_launch(rope_kv4_store_kernel<8, T>, grid, block, 0, stream, 1, p);
+        }
+        return (int)cudaErrorInvalidValue;
+    });
 }
 
 LSB_API int lsb_read_kv4(const void* pages, const int* token_rows, const int* positions, const int* block_table, int table_stride,

@@ -186,6 +186,7 @@ def _p(t: Optional[torch.Tensor]):
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # (device index) -> cudaStream_t as int
+_current_device = torch._C._cuda_getDevice            # (with a CUDA tensor in hand, CUDA is initialised)
 
 
 def _stream(t: torch.Tensor):
@@ -979,11 +980,10 @@ def _check_kv4(what: str, cache, nkv: int, hd: int):
 
 def _same_device(what: str, *tensors) -> None:
     """Refuses tensors of different devices, and a device that is not the current one (its streams take no launches)."""
-    index = tensors[0].get_device()
-    if any(t is not None and t.get_device() != index for t in tensors):
-        raise KernelError(f"{what}: the tensors are on different devices")
-    if index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the tensors are on cuda:{index}, which is not the current device")
+    index = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise KernelError(f"{what}: the tensors are on different devices, or on one that is not the current one (cuda:{index})")
 
 
 def rope_kv4_store(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cache, inv_freq: Optional[torch.Tensor],
