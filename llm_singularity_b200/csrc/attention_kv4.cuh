@@ -40,7 +40,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxSpread = 256;        // requests whose tiles are spread evenly over a grid's blocks
+constexpr int kMaxSpread = 256;        // row tiles (of one kv head, of all requests) whose chunks are spread evenly over a grid's blocks
 constexpr int kMaxSplits = 8;         // blocks of a cluster of portable size
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;        // a row's reference maximum moves when a score exceeds it by this (log2)
@@ -241,26 +241,29 @@ struct Kv4Span {
     }
 };
 
-// SPREAD, for single tokens.  The requests' chunks are one list, and for each kv head and row tile (`items`) as many blocks as fit
-// take an equal stretch of it: whatever the lengths, all blocks end at once.  Neighbouring blocks walk the same tokens of neighbouring
-// heads, whose tiles lie side by side in a page: the pieces of 18 hd bytes that memory is asked for at one time add up to
-// whole pages.  A row tile that a block has from its first chunk to its last is written out by it; of others it leaves maxima,
-// sums and O in its slots (one for what it begins with in the middle, one for what it ends with), which spread_merge_kernel joins.
+// SPREAD.  The chunks of all row tiles of all requests are one list, and for each kv head as many blocks as fit take an equal stretch
+// of it: whatever the lengths, all blocks end at once.  Neighbouring blocks walk the same tokens of neighbouring heads, whose
+// tiles lie side by side in a page: the pieces of 18 hd bytes that memory is asked for at one time add up to whole pages.  A row
+// tile that a block has from its first chunk to its last is written out by it; of others it leaves maxima, sums and O in its
+// slots (one for what it begins with in the middle, one for what it ends with), which spread_merge_kernel joins.
 struct Spread {
-    int items;                                                         // kv heads times row tiles
-    int blocks;                                                        // for each item, no stretch empty (unless there is nothing to do)
+    int blocks;                                                        // for each kv head, no stretch empty (unless there is nothing to do)
     int total;
-    // ends[r]: chunks of requests 0 .. r; filled by all threads of a block
-    __device__ __forceinline__ Spread(const Kv4Params& p, int grid, int* ends, int* warp_sums) {
-        const int tid = threadIdx.x, W = p.window, F = W > 0 ? p.first : 0;
+    // ends[e]: chunks of the row tiles 0 .. e, of which each request has p.row_tiles; filled by all threads of a block
+    __device__ __forceinline__ Spread(const Kv4Params& p, int cols, int grid, int* ends, int* warp_sums) {
+        const int tid = threadIdx.x, W = p.window, F = W > 0 ? p.first : 0, group = p.nh / p.nkv, entries = p.n_requests * p.row_tiles;
         int n[kMaxSpread / 32 / 4], sum = 0;                           // (blocks of at least 128 threads)
         const int each = kMaxSpread / (int)blockDim.x;
 #pragma unroll
         for (int i = 0; i < kMaxSpread / 32 / 4; ++i) {
             if (i >= each) break;
-            const int t = tid * each + i;
+            const int e = tid * each + i, r = e / p.row_tiles, row0 = (e - r * p.row_tiles) * cols;
             n[i] = 0;
-            if (t < p.n_requests && p.q_start[t + 1] - p.q_start[t] == 1) n[i] = Kv4Span(p.kv_len[t] - 1, p.kv_len[t] - 1, W, F).chunks;
+            if (e < entries) {
+                const int q_len = p.q_start[r + 1] - p.q_start[r], rows = q_len * group, base = p.kv_len[r] - q_len;
+                if ((q_len == 1) == (p.mode == 1) && row0 < rows)
+                    n[i] = Kv4Span(base + row0 / group, base + (min(row0 + cols, rows) - 1) / group, W, F).chunks;
+            }
             sum += n[i];
         }
         int upto = sum;
@@ -279,10 +282,9 @@ struct Spread {
             ends[tid * each + i] = upto += n[i];
         }
         __syncthreads();
-        items = p.nkv * p.row_tiles;
         total = ends[kMaxSpread - 1];
         // (a chunk for each warp of a block is the least that is worth joining)
-        blocks = max(1, min(min(grid / items, total), max(p.n_requests, total / kWarps)));
+        blocks = max(1, min(min(grid / p.nkv, total), max(entries, total / kWarps)));
     }
     __device__ __forceinline__ int bound(int block) const { return (int)((long long)block * total / blocks); }
 };
@@ -312,14 +314,12 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
     int r = blockIdx.z, h = blockIdx.y, rt = 0, q_len = 0;
     int at = 0, end = 1;                                               // spread: the block's stretch of the list
     if constexpr (SPREAD) {
-        const Spread list(p, gridDim.x, ends, warp_sums);
-        const int item = (int)blockIdx.x % list.items, part = (int)blockIdx.x / list.items;
+        const Spread list(p, COLS, gridDim.x, ends, warp_sums);
+        const int part = (int)blockIdx.x / p.nkv;
         if (part >= list.blocks) return;
-        h = item / p.row_tiles;
-        rt = item - h * p.row_tiles;
+        h = (int)blockIdx.x - part * p.nkv;
         at = list.bound(part);
         end = list.bound(part + 1);
-        q_len = 1;
     } else {
         q_len = p.q_start[r + 1] - p.q_start[r];
         // (late rows see the most keys, and start first; all blocks of a cluster leave here alike)
@@ -333,15 +333,17 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
   for (; at < end;) {
     int c0, c1;                                                        // the block's chunks of this row tile, of `span.chunks`
     if constexpr (SPREAD) {
-        int lo = 0, hi = p.n_requests - 1;                             // the first request whose chunks end behind `at`
+        int lo = 0, hi = p.n_requests * p.row_tiles - 1;               // the first row tile whose chunks end behind `at`
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (ends[mid] > at) hi = mid; else lo = mid + 1;
         }
-        r = lo;
-        const int before = r > 0 ? ends[r - 1] : 0;
+        const int before = lo > 0 ? ends[lo - 1] : 0;
         c0 = at - before;
-        c1 = min(ends[r] - before, c0 + (end - at));
+        c1 = min(ends[lo] - before, c0 + (end - at));
+        r = lo / p.row_tiles;
+        rt = lo - r * p.row_tiles;
+        q_len = p.q_start[r + 1] - p.q_start[r];
     }
     const int qs = p.q_start[r], n_rows = q_len * group;
     const int row0 = rt * COLS, row1 = min(row0 + COLS, n_rows);
@@ -609,6 +611,14 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             [[maybe_unused]] float total[NT][4];                       // of the chunk's P s, of rows 2 t and 2 t + 1
+            // (32-bit rows: the tensor cores cut their sums off rather than round them, so a chunk's are formed by themselves)
+            [[maybe_unused]] float fresh[NT][2][4];
+            if constexpr (EXACT) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) fresh[n][i >> 2][i & 3] = 0.f;
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const float fa = g % 2 ? high_half(va[u][g / 2]) : low_half(va[u][g / 2]);
@@ -646,13 +656,20 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
                     uint32_t a0 = raised(y), a1 = raised(y >> 4), a2 = raised(z), a3 = raised(z >> 4);
                     if constexpr (EXACT) { a0 = lowered(a0); a1 = lowered(a1); a2 = lowered(a2); a3 = lowered(a3); }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n) {
+                        float(&to)[4] = EXACT ? fresh[n][i - 2 * g] : o[n][i];
 #pragma unroll
                         for (int part = 0; part < PARTS; ++part)
-                            mma(o[n][i], a0, a1, a2, a3, b[n][part][0], b[n][part][1], o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
+                            mma(to, a0, a1, a2, a3, b[n][part][0], b[n][part][1], to[0], to[1], to[2], to[3]);
+                    }
                 }
             }
-            if constexpr (!EXACT) {
+            if constexpr (EXACT) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[n][2 * g + (i >> 2)][i & 3] += fresh[n][i >> 2][i & 3];
+            } else {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -818,11 +835,14 @@ __global__ void __launch_bounds__(128) spread_merge_kernel(const Kv4Params p, in
     __shared__ float4 team_o[TEAMS][UNITS];
     __shared__ float team_m[4], team_l[4];
     lsb_pdl_launch_dependents();
-    const Spread list(p, grid, ends, warp_sums);
-    const int item = blockIdx.x / COLS, c = blockIdx.x % COLS, r = blockIdx.y, tid = threadIdx.x;
-    const int before = r > 0 ? ends[r - 1] : 0, each = ends[r] - before;
-    const int h = item / p.row_tiles, row = (item - h * p.row_tiles) * COLS + c, group = p.nh / p.nkv;
-    if (each == 0 || row >= group) return;                             // (a portion, not a single token; a column without a row)
+    const Spread list(p, COLS, grid, ends, warp_sums);
+    // (Blocks without work leave at once, but one waits: this kernel must not end before the one whose results the next reads.)
+    if (blockIdx.x == 0 && blockIdx.y == 0) lsb_pdl_wait();
+    const int h = blockIdx.x / COLS, c = blockIdx.x % COLS, entry = blockIdx.y, tid = threadIdx.x;
+    const int before = entry > 0 ? ends[entry - 1] : 0, each = ends[entry] - before;
+    const int r = entry / p.row_tiles, qs = p.q_start[r], group = p.nh / p.nkv;
+    const int row = (entry - r * p.row_tiles) * COLS + c;
+    if (each == 0 || row >= (p.q_start[r + 1] - qs) * group) return;   // (not of this launch; a column without a row)
     auto block_of = [&](int x) {                                       // whose stretch holds x
         int b = (int)((long long)x * list.blocks / list.total);
         while (b + 1 < list.blocks && list.bound(b + 1) <= x) ++b;
@@ -832,7 +852,7 @@ __global__ void __launch_bounds__(128) spread_merge_kernel(const Kv4Params p, in
     const int b0 = block_of(before), n = block_of(before + each - 1) - b0 + 1;
     if (n == 1) return;
     lsb_pdl_wait();
-    auto slot_of = [&](int i) { return p.parts + (size_t)(2 * ((b0 + i) * list.items + item) + (i == 0 ? 1 : 0)) * Z::kSlot; };
+    auto slot_of = [&](int i) { return p.parts + (size_t)(2 * ((b0 + i) * p.nkv + h) + (i == 0 ? 1 : 0)) * Z::kSlot; };
     float top = -INFINITY;
     for (int i = tid; i < n; i += 128) top = fmaxf(top, slot_of(i)[c]);
     top = lsb_warp_max(top);
@@ -869,7 +889,7 @@ __global__ void __launch_bounds__(128) spread_merge_kernel(const Kv4Params p, in
         }
         sum = team_l[0] + team_l[1] + team_l[2] + team_l[3];
         const float f = sum == 0.f ? 0.f : 1.f / sum;
-        store_four<T>(reinterpret_cast<T*>(p.out) + (size_t)p.q_start[r] * p.nh * HD + (size_t)(h * group + row) * HD + 4 * tid,
+        store_four<T>(reinterpret_cast<T*>(p.out) + (size_t)(qs + row / group) * p.nh * HD + (size_t)(h * group + row % group) * HD + 4 * tid,
                       make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
     }
 }
@@ -907,7 +927,7 @@ struct Kv4SpreadLaunch {
         if (const int rc = kv4_configure<G, NT, T, true>()) return rc;
         if (const int rc = lsb_launch(attention_kv4_kernel<G, NT, T, true>, dim3(blocks), dim3(kThreads), Kv4Shape<G, NT, T>::kBytes, stream, 1, p))
             return rc;
-        return lsb_launch(spread_merge_kernel<G, NT, T>, dim3(p.nkv * p.row_tiles * 8 * NT, p.n_requests), dim3(128), 0, stream, 1, p, blocks);
+        return lsb_launch(spread_merge_kernel<G, NT, T>, dim3(p.nkv * 8 * NT, p.n_requests * p.row_tiles), dim3(128), 0, stream, 1, p, blocks);
     }
 };
 
@@ -958,10 +978,10 @@ static int kv4_attention(const void* qkv, int qkv_stride, const void* pages, con
     if (n_requests <= 0 || max_rows <= 0) return 0;
     if (splits < 1 || splits > kMaxSplits || eights < 1 || nkv <= 0 || nkv > 65535 || n_requests > 65535 || page_size <= 0 ||
         page_size % kKv4Tile || (long long)num_pages * nkv * (page_size / kKv4Tile) > 0x7fffffffll ||
-        (spread && (mode != 1 || n_requests > kMaxSpread || !parts)))
+        (spread && (mode == 0 || spread < nkv || !parts)))
         return (int)cudaErrorInvalidValue;
     const long long row_tiles = (max_rows + 8 * eights - 1) / (8 * eights);
-    if (row_tiles * splits > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    if (row_tiles * splits > 0x7fffffffll || (spread && row_tiles * n_requests > kMaxSpread)) return (int)cudaErrorInvalidValue;
     Kv4Params p;
     p.qkv = qkv; p.qkv_stride = qkv_stride; p.pages = (const unsigned char*)pages;
     p.q_start = q_start; p.kv_len = kv_len; p.table_rows = table_rows; p.block_table = block_table; p.table_stride = table_stride;

@@ -1041,12 +1041,12 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
     per-request arrays, requests, rows of a request, eights of rows of a block, blocks of a cluster, blocks of a spread launch or
     tiles of an expanded cache, floats of a spread launch's parts).
 
-    Single tokens either have a cluster of blocks to each row tile, or are spread: equal stretches of all chunks of 32 tokens
-    for as many blocks as fit, and a kernel that joins what was cut.  The first ends when the longest context has ended (and has rounds
-    where blocks are more than fit), the second costs about 24 chunks a block more (measured, heads of 64 and 128 in bfloat16: 64
-    requests of 1,000 - 8,100 tokens 147 us with clusters of one, 107 spread; 64 of 4,096 55 and 59; 8 of 4,096 18 and 23;
-    one of 131,072 107 and 50).  A captured launch does not know the lengths: it is spread if the block tables have room for
-    long contexts.
+    Rows either have a cluster of blocks to each row tile, or are spread: equal stretches of all chunks of 32 tokens for as many
+    blocks as fit, and a kernel that joins what was cut.  The first ends when the longest context has ended (and has rounds where
+    blocks are more than fit), the second costs about 24 chunks a block more: rows begun anew, and what was cut joined (measured,
+    heads of 64 and 128: 64 requests of 1,000 - 8,100 tokens 147 us with clusters of one, 100 spread; 64 of 4,096 55 and 59; 8 of
+    4,096 18 and 23; one of 131,072 107 and 50; 40 tokens behind 30,000 145 and 136).  A captured launch does not know
+    the lengths: it is spread if the block tables have room for long contexts.
 
     Portions of 128 tokens and more in bfloat16 with heads of 64 or 128 (mode 3) are expanded: what they see is unpacked once, to an
     ordinary cache, for the tcgen05 prompt kernel (2,011 tokens after 4,096, 32 / 8 heads of 128: 1,000 us where every row tile unpacks
@@ -1084,16 +1084,18 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
             c = rounds * -(-chunks // s) + (2 if s > 1 else 0)
             if cost is None or c < cost:
                 splits, cost = s, c
-        if mode == 1 and R <= 256:
+        row_tiles = -(-rows // (8 * eights))
+        if count * row_tiles <= 256:
             if fixed:
                 even = 0 if capacity >= 4096 else cost
             else:
-                kv = ctx.h_kv_len if n_single == R else ctx.h_kv_len[ctx.h_q_len == 1]
+                of = slice(None) if requests == R else (ctx.h_q_len == 1) == (mode == 1)
+                kv, q = ctx.h_kv_len[of], ctx.h_q_len[of]
                 if window:
-                    kv = kv.clip(max=window + first)
-                even = int(kv.sum()) * (tiles // requests) // (32 * room) + 24
+                    kv = kv.clip(max=window + first + q)
+                even = int((kv * -(-q * group // (8 * eights))).sum()) * nkv // (32 * room) + 24
             if even < cost:
-                spread = max(room, tiles // requests)
+                spread = max(room, nkv)
                 parts = 2 * spread * int(_lib(lib).lsb_attention_kv4_slot(_i(hd), _i(eights)))
         plan.append((mode, 4 * at, count, rows, eights, splits, spread, parts))
     plans[key] = plan
