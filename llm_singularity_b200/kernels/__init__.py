@@ -1085,7 +1085,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
             if cost is None or c < cost:
                 splits, cost = s, c
         row_tiles = -(-rows // (8 * eights))
-        if count * row_tiles <= 256:
+        if count * row_tiles <= 256 and count * row_tiles * chunks < 1 << 31:       # (places in its list of chunks are 32-bit)
             if fixed:
                 even = 0 if capacity >= 4096 else cost
             else:
