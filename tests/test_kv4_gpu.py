@@ -297,6 +297,20 @@ def test_a_page_that_is_not_held_is_reported(ops):
     assert not k[0].any() and not k[2].any() and not v[0].any()
 
 
+def test_the_store_reports_a_negative_position(ops):
+    nh, nkv, hd = 4, 2, 64
+    pages, table = _pool(2, 64, nkv, hd, 16)
+    ctx = step([1, 1], [20, 20])
+    ctx.positions[0] = -17
+    before, qkv = pages.clone(), torch.randn(2, (nh + 2 * nkv) * hd, device="cuda").bfloat16()
+    ops.rope_kv4_store(qkv, nh, nkv, hd, ctx, _view(pages, table, 16), None, 0, torch.empty(2, nh * hd, dtype=qkv.dtype, device="cuda"))
+    with pytest.raises(ops.KernelError, match="page"):
+        ops.check_status()
+    own = table[1, 1].long()
+    assert torch.equal(torch.cat([pages[:own], pages[own + 1:]]), torch.cat([before[:own], before[own + 1:]]))
+    assert not torch.equal(pages[own], before[own])
+
+
 def test_captured_steps_on_growing_contexts_and_another_stream(ops):
     """A step of store and attention, captured once and replayed as the lengths grow, beside the same calls made eagerly on
     another stream."""
