@@ -528,13 +528,23 @@ LSB_API int lsb_prefill_attention_tc5_supported(const void* qkv, int qkv_stride,
 
 template <int HD, typename P>
 static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const P& prm,
-                  dim3 grid, cudaStream_t stream) {
+                  dim3 grid, int fresh_lengths, cudaStream_t stream) {
     static int configured = -1;
     constexpr size_t smem = Smem<HD>::kTotal;
     if (configured < 0)
         configured = (int)cudaFuncSetAttribute(prefill_attention_tc5_kernel<HD, P>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (configured) return configured;
+    if (fresh_lengths) {
+        // Lengths and rows that the kernel before has written are not the metadata that may be read in front of the wait: only that
+        // wait, or a launch without the attribute of lsb_launch, makes that kernel's writes visible.  So the whole kernel starts behind it.
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        return (int)cudaLaunchKernelEx(&cfg, prefill_attention_tc5_kernel<HD, P>, mq, mk, mv, prm);
+    }
     return lsb_launch(prefill_attention_tc5_kernel<HD, P>, grid, dim3(kThreads), smem, stream, 1, mq, mk, mv, prm);
 }
 
@@ -548,7 +558,7 @@ static int prefill(const void* qkv, int qkv_stride, int n_tokens, const void* k_
                                              int n_requests, int max_q_len, int nh, int nkv, int hd, int page_size,
                                              int num_pages, float scale, int window, int skip_single, int sink,
                                              const void* gate, long long gate_stride, float softcap, int linear_bias,
-                                             const float* sink_logit, int first, cudaStream_t stream) {
+                                             const float* sink_logit, int first, int fresh_lengths, cudaStream_t stream) {
     if (n_requests <= 0 || max_q_len <= 0) return 0;
     if (!lsb_prefill_attention_tc5_supported(qkv, qkv_stride, k_pages, v_pages, nh, nkv, hd, page_size) ||
         n_requests > 65535 || (max_q_len + kRows - 1) / kRows > 65535)
@@ -583,9 +593,9 @@ static int prefill(const void* qkv, int qkv_stride, int n_tokens, const void* k_
         FirstParams with;
         static_cast<AttnParams&>(with) = prm;
         with.first = first;
-        return hd == 64 ? launch<64>(mq, mk, mv, with, grid, stream) : launch<128>(mq, mk, mv, with, grid, stream);
+        return hd == 64 ? launch<64>(mq, mk, mv, with, grid, fresh_lengths, stream) : launch<128>(mq, mk, mv, with, grid, fresh_lengths, stream);
     }
-    return hd == 64 ? launch<64>(mq, mk, mv, prm, grid, stream) : launch<128>(mq, mk, mv, prm, grid, stream);
+    return hd == 64 ? launch<64>(mq, mk, mv, prm, grid, fresh_lengths, stream) : launch<128>(mq, mk, mv, prm, grid, fresh_lengths, stream);
 }
 
 LSB_API int lsb_prefill_attention_tc5_biased(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,
@@ -597,19 +607,20 @@ LSB_API int lsb_prefill_attention_tc5_biased(const void* qkv, int qkv_stride, in
                                              const float* sink_logit, cudaStream_t stream) {
     return prefill(qkv, qkv_stride, n_tokens, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out,
                    n_requests, max_q_len, nh, nkv, hd, page_size, num_pages, scale, window, skip_single, sink, gate, gate_stride,
-                   softcap, linear_bias, sink_logit, 0, stream);
+                   softcap, linear_bias, sink_logit, 0, 0, stream);
 }
 
-// `first`: keys before this position stay visible beside the window's.
+// `first`: keys before this position stay visible beside the window's.  `fresh_lengths`: kv_len and table_rows are not the step's
+// own but were written by a kernel of this stream.
 LSB_API int lsb_prefill_attention_tc5_first(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,
                                             const void* v_pages, const int* q_start, const int* kv_len,
                                             const int* table_rows, const int* block_table, int table_stride, void* out,
                                             int n_requests, int max_q_len, int nh, int nkv, int hd, int page_size,
                                             int num_pages, float scale, int window, int skip_single, int first,
-                                            cudaStream_t stream) {
+                                            int fresh_lengths, cudaStream_t stream) {
     return prefill(qkv, qkv_stride, n_tokens, k_pages, v_pages, q_start, kv_len, table_rows, block_table, table_stride, out,
                    n_requests, max_q_len, nh, nkv, hd, page_size, num_pages, scale, window, skip_single, 0, nullptr, 0, 0.f, 0,
-                   nullptr, first, stream);
+                   nullptr, first, fresh_lengths, stream);
 }
 
 LSB_API int lsb_prefill_attention_tc5(const void* qkv, int qkv_stride, int n_tokens, const void* k_pages,

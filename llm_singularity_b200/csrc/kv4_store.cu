@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(128) expand_kv4_kernel(const unsigned char* pa
                                                          const int* block_table, int table_stride, __nv_bfloat16* k_out,
                                                          __nv_bfloat16* v_out, int* table_out, int* rows_out, int* expanded,
                                                          int room, int nkv, int hd, int page_size, int num_pages, int window, int first) {
-    // (The attention behind it reads lengths and rows before it waits, as a step's metadata may be read: it must not start before
-    // they are there, so this kernel lets nothing start early.)
+    // (No early start for the attention behind it, which reads `expanded` and rows_out before anything else: it is launched to begin
+    // when this kernel has ended, lsb_prefill_attention_tc5_first's `fresh_lengths`.)
     const int c = blockIdx.x, h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x;
     const int q_len = q_start[r + 1] - q_start[r], len = kv_len[r], p_lo = len - q_len;
     const int near = (window > 0 && p_lo - window + 1 > 0 ? p_lo - window + 1 : 0) / kKv4Tile;

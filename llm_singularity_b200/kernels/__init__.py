@@ -1141,7 +1141,7 @@ def paged_attention_kv4(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cach
                   _p(its_rows), _p(its_len), count, room, nkv, hd, cache.page_size, pages.shape[0], window, first, _stream(out))
             _call("attention_tc5", "lsb_prefill_attention_tc5_first", _p(qkv), ld, T, _p(kv[0]), _p(kv[1]), per_request[0],
                   _p(its_len), _p(its_rows), _p(its_table), room, _p(out), count, rows // group, nh, nkv, hd, 16, count * room,
-                  _f(scale), window, 1, first, _stream(out))
+                  _f(scale), window, 1, first, 1, _stream(out))        # (1: lengths and rows come from the launch before)
             # (that kernel multiplies the zero weights of hidden places with what is there)
             _call("attention_repair", "lsb_attention_repair", _p(qkv), ld, _p(pages), _p(None), *per_request, _p(table), width, _p(out),
                   count, rows // group, nh, nkv, hd, cache.page_size, pages.shape[0], _f(scale), window, first, 1, _stream(out))
@@ -1176,7 +1176,7 @@ def _attention_with_first(qkv, nh, nkv, hd, ctx, cache, scale, window, first, ou
                        ctypes.c_void_p(ctx.table_rows.data_ptr() + off), _p(cache.block_table), _i(cache.block_table.shape[1]), _p(out),
                        _i(end - begin), _i(ctx.max_q_len))
         _call("attention_tc5", "lsb_prefill_attention_tc5_first", _p(qkv), _i(qkv.shape[1]), _i(ctx.n_tokens), _p(cache.k_pages),
-              _p(cache.v_pages), *per_request, *sizes, _i(1), _i(first), _stream(out))
+              _p(cache.v_pages), *per_request, *sizes, _i(1), _i(first), _i(0), _stream(out))
         # (that kernel multiplies the zero weights of hidden places with what pages hold there)
         _call("attention_repair", "lsb_attention_repair", _p(qkv), _i(qkv.shape[1]), _p(cache.k_pages), _p(cache.v_pages),
               *per_request, *sizes, _i(first), _i(0), _stream(out))

@@ -1,0 +1,64 @@
+"""Which launches attention over a 4-bit cache makes of a step, and with what, without a GPU."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from llm_singularity_b200 import kernels as ops
+from llm_singularity_b200.parts.base import KV4CacheView
+
+ROOM = 296
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Every launch as (entry point, arguments); the checks of devices are off."""
+    made = []
+    monkeypatch.setattr(ops, "_req", lambda t, name, dtype=None, dim=None, contiguous=True: t)
+    monkeypatch.setattr(ops, "_call", lambda lib, fn, *a: made.append((fn, [getattr(x, "value", x) for x in a])))
+    monkeypatch.setattr(ops, "_same_device", lambda what, *t: None)
+    monkeypatch.setattr(ops, "_stream", lambda t: "stream")
+    monkeypatch.setattr(ops, "_kv4_room", lambda *a: ROOM)
+    monkeypatch.setattr(ops, "_lib", lambda name: types.SimpleNamespace(lsb_attention_kv4_slot=lambda *a: 8))
+    return made
+
+
+def _step(q_lens, kv_lens, fixed=False):
+    q, kv = np.array(q_lens, dtype=np.int32), np.array(kv_lens, dtype=np.int32)
+    start = torch.from_numpy(np.concatenate([[0], np.cumsum(q)]).astype(np.int32))
+    return types.SimpleNamespace(n_tokens=int(q.sum()), n_requests=len(q), h_q_len=q, h_kv_len=kv, max_q_len=int(q.max()),
+                                 max_kv_len=int(kv.max()), q_start=start, kv_len=torch.from_numpy(kv),
+                                 table_rows=torch.arange(len(q), dtype=torch.int32), fixed_launch=fixed)
+
+
+def _attend(ctx, nh=8, nkv=2, hd=64, window=0, first=0, dtype=torch.bfloat16, width=None):
+    width = -(-int(ctx.h_kv_len.max()) // 16) if width is None else width
+    cache = KV4CacheView(torch.zeros(3, nkv, 1, 18 * hd, dtype=torch.uint8), torch.zeros(len(ctx.h_q_len), width, dtype=torch.int32), 16,
+                         window or None, 0)
+    q = torch.zeros(ctx.n_tokens, nh * hd, dtype=dtype)
+    ops.paged_attention_kv4(q, nh, nkv, hd, ctx, cache, 0.1, window, torch.empty_like(q), first=first)
+
+
+@pytest.mark.parametrize("window, first", [(0, 0), (50, 0), (50, 4)])
+def test_lengths_written_by_a_launch_are_waited_for(calls, window, first):
+    """The prompt kernel reads a request's length and row before it waits for the launch before it, as it may with a step's own
+    metadata.  Behind the launch that unpacks the cache they are that launch's results: it has to be told, and only then."""
+    ctx = _step([200, 1], [400, 30])
+    _attend(ctx, window=window, first=first)
+    (unpack, of_unpack), (prompt, of_prompt) = [c for c in calls if c[0] in ("lsb_expand_kv4", "lsb_prefill_attention_tc5_first")]
+    its_len, its_rows = of_unpack[10], of_unpack[9]
+    assert (unpack, prompt) == ("lsb_expand_kv4", "lsb_prefill_attention_tc5_first")
+    assert of_prompt[6] == its_len and of_prompt[7] == its_rows and its_len not in (ctx.kv_len.data_ptr(), ctx.table_rows.data_ptr())
+    assert of_prompt[-3:] == [first, 1, "stream"]
+
+
+def test_a_step_s_own_lengths_are_not(calls, monkeypatch):
+    from llm_singularity_b200.parts.base import KVCacheView
+    monkeypatch.setattr(ops, "_lib", lambda name: types.SimpleNamespace(lsb_prefill_attention_tc5_supported=lambda *a: 1))
+    ctx = _step([200], [400])
+    cache = KVCacheView(torch.zeros(3, 2, 16, 64).bfloat16(), torch.zeros(3, 2, 16, 64).bfloat16(), torch.zeros(1, 25, dtype=torch.int32), 16, 50, 0)
+    q = torch.zeros(200, 512).bfloat16()
+    ops.paged_attention(q, 8, 2, 64, ctx, cache, 0.1, 50, torch.empty(200 * 512 + 8).bfloat16()[:200 * 512].view(200, 512), first=4)
+    fn, a = calls[0]
+    assert fn == "lsb_prefill_attention_tc5_first" and a[6] == ctx.kv_len.data_ptr() and a[-3:] == [4, 0, "stream"]
