@@ -34,6 +34,7 @@
 #pragma once
 
 #define LSB_CLUSTER_ALONG_X            // splits are the fastest part of blockIdx.x
+#include "copy_ring.h"
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
     }
     lsb_pdl_wait();
     __syncthreads();
-    uint32_t used = 0;                                                 // chunks that have gone through the warp's ring
+    CopyRing<ST> turn{0};                                              // of the warp's own ring
 
   for (; at < end;) {
     int c0, c1;                                                        // the block's chunks of this row tile, of `span.chunks`
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
     auto issue = [&](int k) {
         if (k >= n_mine) return;
         if (k > 0 && k % 16 == 0) known = places(k);
-        const int place = __shfl_sync(0xffffffffu, known, 2 * (k % 16) + (lane & 1)), s = (used + k) % ST;
+        const int place = __shfl_sync(0xffffffffu, known, 2 * (k % 16) + (lane & 1)), s = turn.stage(k);
         if (lane == 0) bar_expect(&bars[warp][s], Z::kChunk);
         if (lane < 2) bulk_load(ring + s * Z::kChunk + lane * TILE, p.pages + (size_t)place * TILE, TILE, &bars[warp][s]);
     };
@@ -695,12 +696,13 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
     const int k_lo = max(0, ((first_c + 1) / 2 - c0 - warp + kWarps - 1) / kWarps);
     const int k_hi = last_c / 2 - c0 - warp <= 0 ? 0 : (last_c / 2 - c0 - warp + kWarps - 1) / kWarps;
     bool late = false;
+    int k = 0;
 #pragma unroll 1
-    for (int k = 0; k < n_mine; ++k) {
+    for (; k < n_mine; ++k) {
         issue(k + ST - 1);
-        const int stage = (used + k) % ST;
+        const int stage = turn.stage(k);
         uint64_t* bar = &bars[warp][stage];
-        const uint32_t parity = (used + k) / ST & 1u;
+        const uint32_t parity = turn.parity(k);
         if (__any_sync(0xffffffffu, !bar_ready(bar, parity))) {
             late = __any_sync(0xffffffffu, !bar_wait(bar, parity));
             if (late) break;
@@ -711,14 +713,12 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
         __syncwarp();                                                  // the stage may be written over
     }
     if (late) {
-        // a copy did not arrive: what is in flight is waited for (with the same limit) before shared memory goes
+        // chunk k's copy did not arrive: it and those behind it that are under way are waited for (with the same limit) before shared
+        // memory goes
         lsb_set_status(LSB_WAIT_TIMEOUT);
-        for (int i = 0; i < ST; ++i) {
-            const int k = n_mine - 1 - i;
-            if (k >= 0) bar_wait(&bars[warp][(used + k) % ST], (used + k) / ST & 1u);
-        }
+        for (int i = k; i < turn.issued(k, n_mine); ++i) bar_wait(&bars[warp][turn.stage(i)], turn.parity(i));
     }
-    used += max(n_mine, 0);
+    turn.used += max(n_mine, 0);
 
     // ------------------------------------------------------------------ the warps' sums: half of them hand theirs to the others
 #pragma unroll

@@ -68,7 +68,7 @@ SOURCES: Dict[str, object] = {          # library -> its source file (or files)
     "host_runtime": ("host_memory.cpp", "host_scheduler.cpp", "host_step.cpp"),
 }
 HEADERS = ["common.cuh", "attention_tc_noalloc.h", "attention_dv.cuh", "attention_tc5.cuh", "stream_warm.cuh", "gate_act.cuh",
-           "kv4.cuh", "attention_kv4.cuh"]     # of the CUDA libraries
+           "kv4.cuh", "copy_ring.h", "attention_kv4.cuh"]     # of the CUDA libraries
 HOST_HEADERS = ["host_memory.h"]                          # of the host runtime
 
 
