@@ -1066,7 +1066,8 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
         eights = 2 if lib == "attention_kv4" and hd <= 128 and rows > 8 else 1
         tiles = requests * nkv * -(-rows // (8 * eights))
         room = _kv4_room(lib, hd, eights, device)
-        seen = capacity if fixed else ctx.max_kv_len
+        # (the longest of the launch's own requests: one long conversation in the step does not make its prompts long)
+        seen = capacity if fixed else _portion_keys(ctx) if mode == 2 else int(ctx.h_kv_len.max(where=ctx.h_q_len == 1, initial=0))
         if window:
             seen = min(seen, window + most + first)
         chunks = -(-seen // 32)                     # the most of a row tile

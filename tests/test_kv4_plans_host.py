@@ -62,3 +62,22 @@ def test_a_step_s_own_lengths_are_not(calls, monkeypatch):
     ops.paged_attention(q, 8, 2, 64, ctx, cache, 0.1, 50, torch.empty(200 * 512 + 8).bfloat16()[:200 * 512].view(200, 512), first=4)
     fn, a = calls[0]
     assert fn == "lsb_prefill_attention_tc5_first" and a[6] == ctx.kv_len.data_ptr() and a[-3:] == [4, 0, "stream"]
+
+
+def _plan(ctx, hd=128, nh=32, nkv=8, window=0, first=0, capacity=131072, lib="attention_kv4"):
+    return {p[0]: p for p in ops._kv4_plan(ctx, lib, nh, nkv, hd, window, first, capacity, "cuda:0")}
+
+
+def test_a_launch_is_sized_by_its_own_requests(calls):
+    """A conversation of 131,072 tokens beside two prompts of 200: the prompts' unpacked cache has 13 tiles each and two to spare, and
+    few tokens beside a long portion are not split as if they were long."""
+    alone = _plan(_step([200, 200], [200, 200]))
+    beside = _plan(_step([1, 200, 200], [131072, 200, 200]))
+    assert alone[3][6] == beside[3][6] == 15 and set(beside) == {1, 3}
+    lib = "attention_kv4_f32"                                    # (no unpacking there: split over a cluster, or spread)
+    assert _plan(_step([40], [64]), lib=lib)[2][5:] == _plan(_step([1, 40], [131072, 64]), lib=lib)[2][5:]
+    assert _plan(_step([1], [64]), lib=lib)[1][5:] == _plan(_step([1, 40], [64, 131072]), lib=lib)[1][5:]
+
+
+def test_a_captured_launch_is_sized_by_the_table(calls):
+    assert _plan(_step([200], [200], fixed=True), capacity=1600)[3][6] == 102
