@@ -1091,7 +1091,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
                 even = 0 if capacity >= 4096 else cost
             else:
                 of = slice(None) if requests == R else (ctx.h_q_len == 1) == (mode == 1)
-                kv, q = ctx.h_kv_len[of], ctx.h_q_len[of]
+                kv, q = ctx.h_kv_len[of].astype("int64"), ctx.h_q_len[of].astype("int64")    # (a window and first tokens reach 2^31)
                 if window:
                     kv = kv.clip(max=window + first + q)
                 even = int((kv * -(-q * group // (8 * eights))).sum()) * nkv // (32 * room) + 24

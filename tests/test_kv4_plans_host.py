@@ -81,3 +81,10 @@ def test_a_launch_is_sized_by_its_own_requests(calls):
 
 def test_a_captured_launch_is_sized_by_the_table(calls):
     assert _plan(_step([200], [200], fixed=True), capacity=1600)[3][6] == 102
+
+
+@pytest.mark.parametrize("lib", ["attention_kv4", "attention_kv4_f32"])
+@pytest.mark.parametrize("q_lens, kv_lens", [([1], [64]), ([1] * 8, [4096] * 8), ([40], [64]), ([1] * 64, list(range(1000, 7400, 100)))])
+def test_a_window_wider_than_any_context_changes_no_plan(calls, lib, q_lens, kv_lens):
+    far = dict(window=(1 << 30) - 1, first=1 << 30)
+    assert _plan(_step(q_lens, kv_lens), lib=lib, **far) == _plan(_step(q_lens, kv_lens), lib=lib)
