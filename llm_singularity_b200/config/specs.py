@@ -576,7 +576,8 @@ KV_CACHES = {"compute": None, "int4": 4}          # how keys and values may be c
 def with_long_context(spec: ModelSpec, kv_cache: str = "compute", window: Optional[int] = None, first_tokens: int = 0) -> ModelSpec:
     """``spec`` as it is served with other caches: keys and values held as ``kv_cache`` says, and, with a ``window``, every
     query seeing the last ``window`` tokens and the first ``first_tokens`` only, so that a sequence may grow without end in
-    bounded memory.  For models whose layers all mix by ``AttentionSpec``; others have caches of their own."""
+    bounded memory.  A layer that has a window of its own sees no more than it did: the narrower of the two, and no first tokens
+    but those that it has always seen.  For models whose layers all mix by ``AttentionSpec``; others have caches of their own."""
     if kv_cache not in KV_CACHES:
         raise ValueError(f"kv_cache must be one of {sorted(KV_CACHES)}, got {kv_cache!r}")
     if window is not None and window < 1:
@@ -589,7 +590,12 @@ def with_long_context(spec: ModelSpec, kv_cache: str = "compute", window: Option
     if other is not None:
         raise ValueError(f"{spec.architecture}: 4-bit caches and windows can be asked for where every layer is plain "
                          f"attention; this model has '{other}'")
-    change = dict(cache_bits=KV_CACHES[kv_cache])
-    if window is not None:
-        change.update(window=window, first_tokens=first_tokens)
-    return replace(spec, blocks=tuple(replace(b, mixer=replace(b.mixer, **change)) for b in spec.blocks))
+    def changed(mixer: AttentionSpec) -> AttentionSpec:
+        mixer = replace(mixer, cache_bits=KV_CACHES[kv_cache])
+        if window is None:
+            return mixer
+        if mixer.window is None:
+            return replace(mixer, window=window, first_tokens=first_tokens)
+        return replace(mixer, window=min(window, mixer.window), first_tokens=min(first_tokens, mixer.first_tokens or 0))
+
+    return replace(spec, blocks=tuple(replace(b, mixer=changed(b.mixer)) for b in spec.blocks))
