@@ -580,10 +580,10 @@ def with_long_context(spec: ModelSpec, kv_cache: str = "compute", window: Option
     but those that it has always seen.  For models whose layers all mix by ``AttentionSpec``; others have caches of their own."""
     if kv_cache not in KV_CACHES:
         raise ValueError(f"kv_cache must be one of {sorted(KV_CACHES)}, got {kv_cache!r}")
-    if window is not None and window < 1:
-        raise ValueError(f"window must be at least 1, got {window}")
-    if first_tokens < 0 or (first_tokens and window is None):
-        raise ValueError(f"first_tokens {first_tokens} must not be negative, and goes with a window")
+    if window is not None and not 1 <= window <= 1 << 30:              # (lengths are 32-bit in the cache's tables and the kernels)
+        raise ValueError(f"window must be at least 1 and at most 2^30, got {window}")
+    if not 0 <= first_tokens <= 1 << 30 or (first_tokens and window is None):
+        raise ValueError(f"first_tokens {first_tokens} must not be negative or above 2^30, and goes with a window")
     if kv_cache == "compute" and window is None:
         return spec
     other = next((b.mixer.kind for b in spec.blocks if not isinstance(getattr(b, "mixer", None), AttentionSpec)), None)

@@ -36,3 +36,12 @@ def test_no_layer_sees_more_than_it_did(own, window, first):
 def test_without_a_window_layers_keep_theirs():
     own = [(512, None), (None, None)]
     assert _rules(with_long_context(_spec(*own), "int4"))[:2] == own
+
+
+@pytest.mark.parametrize("window, first, says", [(2 ** 32 + 5, 0, "window"), (2 ** 31, 0, "window"), (2 ** 30 + 1, 0, "window"),
+                                                 (8, 2 ** 30 + 1, "first_tokens"), (8, 2 ** 64 + 1, "first_tokens")])
+def test_lengths_of_more_than_30_bits_are_refused(window, first, says):
+    """(Cut to 32 bits, a window of 2^32 + 5 would be one of 5.)"""
+    with pytest.raises(ValueError, match=says):
+        with_long_context(_spec(), "compute", window, first)
+    assert _rules(with_long_context(_spec(), "compute", 2 ** 30, 2 ** 30))[0] == (2 ** 30, 2 ** 30)
