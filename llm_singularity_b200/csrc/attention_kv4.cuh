@@ -937,14 +937,18 @@ struct Kv4SpreadLaunch {
     }
 };
 
-// Blocks that an SM holds at once (of either form; they take the same).
+// Blocks of a form that an SM holds at once.  The spread one has up to 30 registers more: with heads of 64 and 16 rows two fit where three
+// of the other do, with heads of 32 and 8 rows four where five do.  (Stretches for the other's number of blocks run in two rounds: one
+// token at 131,072, 32 / 2 heads of 64, 36.9 us where it takes 26.6; 64 at 1,000 - 8,100, 32 / 8 of 32, 67.6 and 55.3.)
 struct Kv4Room {
-    template <int G, int NT, typename T> int run() const {
+    bool spread;
+    template <int G, int NT, typename T, bool SPREAD> static int of() {
         int got = 0;
-        if (kv4_configure<G, NT, T, false>()) return 0;
-        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, attention_kv4_kernel<G, NT, T, false>, kThreads,
+        if (kv4_configure<G, NT, T, SPREAD>()) return 0;
+        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, attention_kv4_kernel<G, NT, T, SPREAD>, kThreads,
                                                              Kv4Shape<G, NT, T>::kBytes) == cudaSuccess ? got : 0;
     }
+    template <int G, int NT, typename T> int run() const { return spread ? of<G, NT, T, true>() : of<G, NT, T, false>(); }
 };
 
 struct Kv4SlotFloats {
@@ -1009,8 +1013,8 @@ static int kv4_attention(const void* qkv, int qkv_stride, const void* pages, con
                                 n_requests, max_rows, nh, nkv, hd, page_size, num_pages, scale, window, first, mode,         \
                                 eights, splits, spread, parts, stream);                                                      \
     }                                                                                                                        \
-    LSB_API int lsb_attention_kv4_room(int hd, int eights) {                                                                 \
-        const int got = kv4_of<T>(hd, eights, Kv4Room{});                                                                    \
+    LSB_API int lsb_attention_kv4_room(int hd, int eights, int spread) {                                                     \
+        const int got = kv4_of<T>(hd, eights, Kv4Room{spread != 0});                                                         \
         return got < 0 ? 0 : got;                                                                                            \
     }                                                                                                                        \
     LSB_API int lsb_attention_kv4_slot(int hd, int eights) { return kv4_of<T>(hd, eights, Kv4SlotFloats{}); }

@@ -1028,11 +1028,11 @@ def read_kv4(cache, nkv: int, hd: int, token_rows: torch.Tensor, positions: torc
 _kv4_rooms: Dict[tuple, int] = {}
 
 
-def _kv4_room(lib: str, hd: int, eights: int, device) -> int:
-    """Blocks of a kernel that the device holds at once."""
-    key = (lib, hd, eights, device)
+def _kv4_room(lib: str, hd: int, eights: int, spread: int, device) -> int:
+    """Blocks of a kernel, in clusters or spread (the two have registers of their own), that the device holds at once."""
+    key = (lib, hd, eights, spread, device)
     if key not in _kv4_rooms:
-        _kv4_rooms[key] = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights))) * num_sms(device)
+        _kv4_rooms[key] = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights), _i(spread))) * num_sms(device)
     return _kv4_rooms[key]
 
 
@@ -1065,7 +1065,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
         rows = most * group
         eights = 2 if lib == "attention_kv4" and hd <= 128 and rows > 8 else 1
         tiles = requests * nkv * -(-rows // (8 * eights))
-        room = _kv4_room(lib, hd, eights, device)
+        room, evenly = (_kv4_room(lib, hd, eights, form, device) for form in (0, 1))
         # (the longest of the launch's own requests: one long conversation in the step does not make its prompts long)
         seen = capacity if fixed else _portion_keys(ctx) if mode == 2 else int(ctx.h_kv_len.max(where=ctx.h_q_len == 1, initial=0))
         if window:
@@ -1094,9 +1094,9 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
                 kv, q = ctx.h_kv_len[of].astype("int64"), ctx.h_q_len[of].astype("int64")    # (a window and first tokens reach 2^31)
                 if window:
                     kv = kv.clip(max=window + first + q)
-                even = int((kv * -(-q * group // (8 * eights))).sum()) * nkv // (32 * room) + 24
+                even = int((kv * -(-q * group // (8 * eights))).sum()) * nkv // (32 * evenly) + 24
             if even < cost:
-                spread = max(room, nkv)
+                spread = max(evenly, nkv)
                 parts = 2 * spread * int(_lib(lib).lsb_attention_kv4_slot(_i(hd), _i(eights)))
         plan.append((mode, 4 * at, count, rows, eights, splits, spread, parts))
     plans[key] = plan

@@ -88,3 +88,10 @@ def test_a_captured_launch_is_sized_by_the_table(calls):
 def test_a_window_wider_than_any_context_changes_no_plan(calls, lib, q_lens, kv_lens):
     far = dict(window=(1 << 30) - 1, first=1 << 30)
     assert _plan(_step(q_lens, kv_lens), lib=lib, **far) == _plan(_step(q_lens, kv_lens), lib=lib)
+
+
+def test_a_spread_launch_has_the_blocks_that_fit_of_its_own_kernel(calls, monkeypatch):
+    """The kernel that spreads chunks has more registers than the one with clusters, and fewer of its blocks fit."""
+    monkeypatch.setattr(ops, "_kv4_room", lambda lib, hd, eights, spread, device: 296 if spread else 444)
+    for ctx in (_step([1], [131072]), _step([1] * 8, [9000] * 8, fixed=True)):
+        assert _plan(ctx, hd=64, nh=32, nkv=2)[1][6] == 296                 # 16 rows a block
