@@ -1046,7 +1046,10 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
     blocks are more than fit), the second costs about 24 chunks a block more: rows begun anew, and what was cut joined (measured,
     heads of 64 and 128: 64 requests of 1,000 - 8,100 tokens 147 us with clusters of one, 100 spread; 64 of 4,096 55 and 59; 8 of
     4,096 18 and 23; one of 131,072 107 and 50; 40 tokens behind 30,000 145 and 136).  A captured launch does not know
-    the lengths: it is spread if the block tables have room for long contexts.
+    the lengths: where a window bounds what a request sees it is planned for that, and spread otherwise if the block tables have room for
+    long contexts.  (Captured and replayed, heads of 64, with clusters and spread: window 1,024, 8 tokens 16.4 us and 20.2, 64 24.6 and
+    36.9.  Without a window 8 of 4,096 20.5 and 24.6, 64 of 1,000 22.5 and 36.9, but clusters of a captured launch that meets one
+    long context among short ones take as long as a block needs for it.)
 
     Portions of 128 tokens and more in bfloat16 with heads of 64 or 128 (mode 3) are expanded: what they see is unpacked once, to an
     ordinary cache, for the tcgen05 prompt kernel (2,011 tokens after 4,096, 32 / 8 heads of 128: 1,000 us where every row tile unpacks
@@ -1087,8 +1090,10 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
                 splits, cost = s, c
         row_tiles = -(-rows // (8 * eights))
         if count * row_tiles <= 256 and count * row_tiles * chunks < 1 << 31:       # (places in its list of chunks are 32-bit)
-            if fixed:
+            if fixed and not window:
                 even = 0 if capacity >= 4096 else cost
+            elif fixed:                             # as if every request were past its window
+                even = requests * row_tiles * seen * nkv // (32 * evenly) + 24
             else:
                 of = slice(None) if requests == R else (ctx.h_q_len == 1) == (mode == 1)
                 kv, q = ctx.h_kv_len[of].astype("int64"), ctx.h_q_len[of].astype("int64")    # (a window and first tokens reach 2^31)

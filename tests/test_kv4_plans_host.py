@@ -95,3 +95,12 @@ def test_a_spread_launch_has_the_blocks_that_fit_of_its_own_kernel(calls, monkey
     monkeypatch.setattr(ops, "_kv4_room", lambda lib, hd, eights, spread, device: 296 if spread else 444)
     for ctx in (_step([1], [131072]), _step([1] * 8, [9000] * 8, fixed=True)):
         assert _plan(ctx, hd=64, nh=32, nkv=2)[1][6] == 296                 # 16 rows a block
+
+
+@pytest.mark.parametrize("requests, window, first", [(1, 1024, 4), (8, 1024, 4), (64, 1024, 4), (32, 4000, 0), (8, 100000, 4), (1, 100000, 0)])
+def test_a_captured_launch_with_a_window_is_planned_for_it(calls, requests, window, first):
+    """However wide the block tables are, a request is seen in its window only: the plan is that of a step of requests past it."""
+    captured = _plan(_step([1] * requests, [5] * requests, fixed=True), hd=64, window=window, first=first)[1]
+    eager = _plan(_step([1] * requests, [131072] * requests), hd=64, window=window, first=first)[1]
+    assert captured[5:] == eager[5:] and (captured[6] == 0) == (window < 5000)
+    assert _plan(_step([1] * requests, [5] * requests, fixed=True), hd=64)[1][6] > 0
