@@ -937,18 +937,36 @@ struct Kv4SpreadLaunch {
     }
 };
 
-// Blocks of a form that an SM holds at once.  The spread one has up to 30 registers more: with heads of 64 and 16 rows two fit where three
-// of the other do, with heads of 32 and 8 rows four where five do.  (Stretches for the other's number of blocks run in two rounds: one
-// token at 131,072, 32 / 2 heads of 64, 36.9 us where it takes 26.6; 64 at 1,000 - 8,100, 32 / 8 of 32, 67.6 and 55.3.)
+// What fits at once: (form 0) blocks on an SM, (1) of the kernel that spreads, or clusters of `form` blocks on the device.  The spread form has
+// up to 30 registers more: with heads of 64 and 16 rows two blocks fit where three of the other do, with heads of 32 and 8 rows four where
+// five do.  (Stretches for the other's number of blocks run in two rounds: one token at 131,072, 32 / 2 heads of 64, 36.9 us where it
+// takes 26.6; 64 at 1,000 - 8,100, 32 / 8 of 32, 67.6 and 55.3.)  A cluster's blocks share a group of SMs, whose places clusters of 5 to 8
+// blocks do not fill: of 296 blocks' places 40 clusters of 7 take two rounds (40 tokens behind 30,000, 16 / 1 heads of 128: 121 us, spread
+// 72).
 struct Kv4Room {
-    bool spread;
-    template <int G, int NT, typename T, bool SPREAD> static int of() {
+    int form;
+    template <int G, int NT, typename T, bool SPREAD> static int blocks() {
         int got = 0;
         if (kv4_configure<G, NT, T, SPREAD>()) return 0;
         return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, attention_kv4_kernel<G, NT, T, SPREAD>, kThreads,
                                                              Kv4Shape<G, NT, T>::kBytes) == cudaSuccess ? got : 0;
     }
-    template <int G, int NT, typename T> int run() const { return spread ? of<G, NT, T, true>() : of<G, NT, T, false>(); }
+    template <int G, int NT, typename T> int run() const {
+        if (form < 2) return form ? blocks<G, NT, T, true>() : blocks<G, NT, T, false>();
+        if (kv4_configure<G, NT, T, false>()) return 0;
+        cudaLaunchAttribute along;
+        along.id = cudaLaunchAttributeClusterDimension;
+        along.val.clusterDim.x = form;
+        along.val.clusterDim.y = along.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(form);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = Kv4Shape<G, NT, T>::kBytes;
+        cfg.attrs = &along;
+        cfg.numAttrs = 1;
+        int got = 0;
+        return cudaOccupancyMaxActiveClusters(&got, attention_kv4_kernel<G, NT, T, false>, &cfg) == cudaSuccess ? got : 0;
+    }
 };
 
 struct Kv4SlotFloats {
@@ -1013,8 +1031,8 @@ static int kv4_attention(const void* qkv, int qkv_stride, const void* pages, con
                                 n_requests, max_rows, nh, nkv, hd, page_size, num_pages, scale, window, first, mode,         \
                                 eights, splits, spread, parts, stream);                                                      \
     }                                                                                                                        \
-    LSB_API int lsb_attention_kv4_room(int hd, int eights, int spread) {                                                     \
-        const int got = kv4_of<T>(hd, eights, Kv4Room{spread != 0});                                                         \
+    LSB_API int lsb_attention_kv4_room(int hd, int eights, int form) {                                                       \
+        const int got = form < 0 || form > kMaxSplits ? -1 : kv4_of<T>(hd, eights, Kv4Room{form});                           \
         return got < 0 ? 0 : got;                                                                                            \
     }                                                                                                                        \
     LSB_API int lsb_attention_kv4_slot(int hd, int eights) { return kv4_of<T>(hd, eights, Kv4SlotFloats{}); }

@@ -1028,11 +1028,12 @@ def read_kv4(cache, nkv: int, hd: int, token_rows: torch.Tensor, positions: torc
 _kv4_rooms: Dict[tuple, int] = {}
 
 
-def _kv4_room(lib: str, hd: int, eights: int, spread: int, device) -> int:
-    """Blocks of a kernel, in clusters or spread (the two have registers of their own), that the device holds at once."""
-    key = (lib, hd, eights, spread, device)
+def _kv4_room(lib: str, hd: int, eights: int, form: int, device) -> int:
+    """What the device holds at once: 0: blocks that have a row tile each; 1: blocks of the kernel that spreads, which has registers of
+    its own; 2 and more: clusters of so many blocks."""
+    key = (lib, hd, eights, form, device)
     if key not in _kv4_rooms:
-        _kv4_rooms[key] = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights), _i(spread))) * num_sms(device)
+        _kv4_rooms[key] = int(_lib(lib).lsb_attention_kv4_room(_i(hd), _i(eights), _i(form))) * (1 if form > 1 else num_sms(device))
     return _kv4_rooms[key]
 
 
@@ -1068,7 +1069,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
         rows = most * group
         eights = 2 if lib == "attention_kv4" and hd <= 128 and rows > 8 else 1
         tiles = requests * nkv * -(-rows // (8 * eights))
-        room, evenly = (_kv4_room(lib, hd, eights, form, device) for form in (0, 1))
+        evenly = _kv4_room(lib, hd, eights, 1, device)
         # (the longest of the launch's own requests: one long conversation in the step does not make its prompts long)
         seen = capacity if fixed else _portion_keys(ctx) if mode == 2 else int(ctx.h_kv_len.max(where=ctx.h_q_len == 1, initial=0))
         if window:
@@ -1082,7 +1083,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
                 continue
         cost = None
         for s in range(1, 9):
-            rounds = -(-tiles * s // room)
+            rounds = -(-tiles // max(1, _kv4_room(lib, hd, eights, s if s > 1 else 0, device)))
             if s > 1 and (rounds > 1 or 4 * (s - 1) >= chunks):
                 break
             c = rounds * -(-chunks // s) + (2 if s > 1 else 0)

@@ -19,7 +19,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(ops, "_call", lambda lib, fn, *a: made.append((fn, [getattr(x, "value", x) for x in a])))
     monkeypatch.setattr(ops, "_same_device", lambda what, *t: None)
     monkeypatch.setattr(ops, "_stream", lambda t: "stream")
-    monkeypatch.setattr(ops, "_kv4_room", lambda *a: ROOM)
+    monkeypatch.setattr(ops, "_kv4_room", lambda lib, hd, eights, form, device: ROOM // max(1, form))
     monkeypatch.setattr(ops, "_lib", lambda name: types.SimpleNamespace(lsb_attention_kv4_slot=lambda *a: 8))
     return made
 
@@ -104,3 +104,11 @@ def test_a_captured_launch_with_a_window_is_planned_for_it(calls, requests, wind
     eager = _plan(_step([1] * requests, [131072] * requests), hd=64, window=window, first=first)[1]
     assert captured[5:] == eager[5:] and (captured[6] == 0) == (window < 5000)
     assert _plan(_step([1] * requests, [5] * requests, fixed=True), hd=64)[1][6] > 0
+
+
+def test_clusters_are_counted_by_those_that_fit(calls, monkeypatch):
+    """Blocks of 296 places may be 40 clusters of 7 by number, but where only 34 fit they take two rounds: fewer splits, or spread."""
+    monkeypatch.setattr(ops, "_kv4_room", lambda lib, hd, eights, form, device: {0: 296, 1: 296, 2: 148, 3: 96, 4: 72, 5: 56, 6: 46, 7: 34, 8: 34}[form])
+    at = lambda requests, nkv: _plan(_step([1] * requests, [1500] * requests), nh=nkv, nkv=nkv)[1][5:7]
+    assert at(5, 8) == (6, 0)                                    # 40 row tiles
+    assert at(4, 8) == (8, 0) and at(34, 1) == (8, 0) and at(35, 1) == (6, 0)
