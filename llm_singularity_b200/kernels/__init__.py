@@ -1044,9 +1044,11 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
 
     Rows either have a cluster of blocks to each row tile, or are spread: equal stretches of all chunks of 32 tokens for as many
     blocks as fit, and a kernel that joins what was cut.  The first ends when the longest context has ended (and has rounds where
-    blocks are more than fit), the second costs about 24 chunks a block more: rows begun anew, and what was cut joined (measured,
-    heads of 64 and 128: 64 requests of 1,000 - 8,100 tokens 147 us with clusters of one, 100 spread; 64 of 4,096 55 and 59; 8 of
-    4,096 18 and 23; one of 131,072 107 and 50; 40 tokens behind 30,000 145 and 136).  A captured launch does not know
+    clusters are more than fit), the second costs the time of about 20 chunks more, to join what was cut, and of 24 for each row tile that
+    a block begins.  (Over 174 shapes of single tokens and short portions, heads of 32 to 256, both types: on average 0.4 % slower than
+    the better of the two.  Heads of 128, 32 / 8, clusters and spread: 64 requests of 1,000 - 8,100 tokens 124 us and 96; 64 of
+    4,096 90 and 88; 64 of 300 - 1,000 26.4 and 32.5; 8 of 4,096 18.9 and 21.8; one of 131,072 130 and 46; 40 tokens behind 30,000 139
+    and 126; 40 behind 2,000 20.2 and 25.9.)  A captured launch does not know
     the lengths: where a window bounds what a request sees it is planned for that, and spread otherwise if the block tables have room for
     long contexts.  (Captured and replayed, heads of 64, with clusters and spread: window 1,024, 8 tokens 16.4 us and 20.2, 64 24.6 and
     36.9.  Without a window 8 of 4,096 20.5 and 24.6, 64 of 1,000 22.5 and 36.9, but clusters of a captured launch that meets one
@@ -1089,18 +1091,18 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
             c = rounds * -(-chunks // s) + (2 if s > 1 else 0)
             if cost is None or c < cost:
                 splits, cost = s, c
-        row_tiles = -(-rows // (8 * eights))
+        row_tiles, join = -(-rows // (8 * eights)), 20 + 24 * tiles // evenly
         if count * row_tiles <= 256 and count * row_tiles * chunks < 1 << 31:       # (places in its list of chunks are 32-bit)
             if fixed and not window:
                 even = 0 if capacity >= 4096 else cost
             elif fixed:                             # as if every request were past its window
-                even = requests * row_tiles * seen * nkv // (32 * evenly) + 24
+                even = requests * row_tiles * seen * nkv // (32 * evenly) + join
             else:
                 of = slice(None) if requests == R else (ctx.h_q_len == 1) == (mode == 1)
                 kv, q = ctx.h_kv_len[of].astype("int64"), ctx.h_q_len[of].astype("int64")    # (a window and first tokens reach 2^31)
                 if window:
                     kv = kv.clip(max=window + first + q)
-                even = int((kv * -(-q * group // (8 * eights))).sum()) * nkv // (32 * evenly) + 24
+                even = int((kv * -(-q * group // (8 * eights))).sum()) * nkv // (32 * evenly) + join
             if even < cost:
                 spread = max(evenly, nkv)
                 parts = 2 * spread * int(_lib(lib).lsb_attention_kv4_slot(_i(hd), _i(eights)))

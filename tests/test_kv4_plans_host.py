@@ -112,3 +112,12 @@ def test_clusters_are_counted_by_those_that_fit(calls, monkeypatch):
     at = lambda requests, nkv: _plan(_step([1] * requests, [1500] * requests), nh=nkv, nkv=nkv)[1][5:7]
     assert at(5, 8) == (6, 0)                                    # 40 row tiles
     assert at(4, 8) == (8, 0) and at(34, 1) == (8, 0) and at(35, 1) == (6, 0)
+
+
+def test_many_short_requests_are_not_spread(calls, monkeypatch):
+    """What a block begins anew counts: 64 requests of up to 1,000 tokens run faster a block each, of up to 8,100 spread."""
+    monkeypatch.setattr(ops, "_kv4_room", lambda lib, hd, eights, form, device: 444 // max(1, form))
+    lens = lambda lo, hi: [lo + (hi - lo) * ((7 * i + 3) % 64) // 63 for i in range(64)]
+    assert _plan(_step([1] * 64, lens(300, 1000)))[1][6] == 0
+    assert _plan(_step([1] * 64, lens(1000, 8100)))[1][6] == 444
+    assert _plan(_step([1] * 64, [9000] * 64), window=1024, first=4)[1][6] == 0
