@@ -63,7 +63,7 @@ struct Kv4Params {
     int nh, nkv, tiles_per_page, num_pages;
     float scale;
     int window, first;
-    int mode;                          // 0: every request; 1: those that bring one token; 2: the others
+    int mode;                          // which requests: 1: those that bring one token; 2: the others
     int splits;
     float* parts;                      // spread: what blocks have of rows that others have a part of, two slots a block
     int n_requests, row_tiles;         // spread: all of them; of each request
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, Kv4Shape<G, NT, T>::kBlocks) attenti
         q_len = p.q_start[r + 1] - p.q_start[r];
         // (late rows see the most keys, and start first; all blocks of a cluster leave here alike)
         rt = (q_len * group + COLS - 1) / COLS - 1 - (int)(blockIdx.x / splits);
-        if (rt < 0 || (p.mode == 1 && q_len != 1) || (p.mode == 2 && q_len == 1)) return;
+        if (rt < 0 || (q_len == 1) != (p.mode == 1)) return;
     }
     lsb_pdl_wait();
     __syncthreads();
@@ -1006,7 +1006,7 @@ static int kv4_attention(const void* qkv, int qkv_stride, const void* pages, con
     if (n_requests <= 0 || max_rows <= 0) return 0;
     if (splits < 1 || splits > kMaxSplits || eights < 1 || nkv <= 0 || nkv > 65535 || n_requests > 65535 || page_size <= 0 ||
         page_size % kKv4Tile || (long long)num_pages * nkv * (page_size / kKv4Tile) > 0x7fffffffll ||
-        (spread && (mode == 0 || spread < nkv || !parts)))
+        (mode != 1 && mode != 2) || (spread && (spread < nkv || !parts)))
         return (int)cudaErrorInvalidValue;
     const long long row_tiles = (max_rows + 8 * eights - 1) / (8 * eights);
     if (row_tiles * splits > 0x7fffffffll || (spread && row_tiles * n_requests > kMaxSpread)) return (int)cudaErrorInvalidValue;
