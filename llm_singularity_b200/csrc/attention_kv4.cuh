@@ -17,8 +17,10 @@
 // 8 x 8 transposition of bfloat16 (movmatrix) per eight tokens, rows and group.
 // A code becomes a number by masking it into the mantissa of a power of two.  Keys, as float16: of a word's four nibbles to a half
 // two need no shift (1024 + c and 1024 + 16 c, whose row takes a sixteenth of its dim), and what is too much is taken off the
-// accumulator's start, a sum over the row's dims: 32 products of one group, so at most 2^-11 of the group's largest product is
-// lost.  Rows are scaled by a power of two for it, their largest dim to [16, 32).  Values, as bfloat16 (a probability times a scale
+// accumulator's start, a sum over the row's dims.  So an accumulator holds up to 1,039 times the sum of the row's magnitudes in a group
+// on its way to a product that may be much less, and each of a dozen additions may lose about 2^-24 of that.  (A choice of speed, and less than
+// the worst by far: with scores of up to 1,400, large parts of them common to all keys, results were no further from 64 bits than
+// the rounding of the result.)  Rows are scaled by a power of two for it, their largest dim to [16, 32).  Values, as bfloat16 (a probability times a scale
 // has no bounds): 128 + c, and 136 times the sum of a chunk's weights (a product with ones) is taken off the sums after each
 // chunk of 32 tokens, before it could add up over all of them.
 // 32-bit rows: queries and probabilities are sums of three bfloat16 (24 bits), and 136 is subtracted from codes before the
@@ -28,9 +30,11 @@
 // Nothing but a warp's own barriers orders that ring; warps and blocks meet once, at the end of a row tile.
 //
 // Measured: 64 requests of 1,000 - 8,100 tokens, 32 / 8 heads of 128, 93 us, 3.6 TB/s of codes and scales, 55 % of what a copy
-// reaches; the loads alone, without the products, take 73 - 81 (pieces of 4.6 KB, whatever the ring's depth), and the issue of
-// instructions nearly as long, 350 a tile.  One request of 131,072 tokens: 44 us, 3.4 TB/s.  Portions of few rows are bound by the
-// instructions that unpack a code for each row tile: 40 tokens behind 30,000, 127 us.  32-bit rows cost three products for one.
+// reaches; one request of 131,072 tokens 44 us, 3.4 TB/s.  There DRAM is at 45 %, half of the issue slots and of the integer pipe are
+// used, and the 12 warps that registers let an SM hold wait for their own instructions most, 320 a tile.  The loads alone, without the
+// products, take 73 - 81 us of the 93 (two copies of 2,304 bytes a chunk, whatever the ring's depth).  Portions of few rows are bound by
+// the same instructions, which unpack a code again for each row tile: 40 tokens behind 30,000, 125 us, DRAM at 3 %, the tensor cores
+// at 37 %.  32-bit rows cost three products for one.
 #pragma once
 
 #define LSB_CLUSTER_ALONG_X            // splits are the fastest part of blockIdx.x

@@ -7,9 +7,10 @@
 // a border, and 32-bit angles are off by up to 2^-24 of themselves, 0.008 at position 131,072.  Queries take the 64-bit angle's
 // sine and cosine in 32-bit.  The angles are shared by a token's heads.
 //
-// One block per token; keys and values leave as 9/32 of their bfloat16 bytes.  What bounds it is the issue of instructions, about
-// 775 a warp: 2,011 tokens of 32 / 8 heads of 128 take 21.5 us where their bytes would take 6.6.  (With a head size known at
-// launch only, a 64-bit division per code and keys passed through shared memory it took 27.)  A step of single tokens is a
+// One block per token; keys and values leave as 9/32 of their bfloat16 bytes.  2,011 tokens of 32 / 8 heads of 128 take 21.5 us where
+// their bytes would take 6.6: a block's start (its position, 64-bit sines, a barrier) comes before its first load, and then that load is
+// waited for; 57 % of issue slots (775 instructions a warp), 54 % of an SM's warps and 13 % of DRAM are in use.  (With a head size known
+// at launch only, a 64-bit division per code and keys passed through shared memory it took 27.)  A step of single tokens is a
 // launch: 3 us.
 #include "kv4.cuh"
 

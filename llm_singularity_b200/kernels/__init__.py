@@ -1057,7 +1057,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
     Portions of 128 tokens and more in bfloat16 with heads of 64 or 128 (mode 3) are expanded: what they see is unpacked once, to an
     ordinary cache, for the tcgen05 prompt kernel (2,011 tokens after 4,096, 32 / 8 heads of 128: 1,000 us where every row tile unpacks
     for itself, 229 us so), as long as that cache stays within 1 GB (256 MB in a captured step, which has to have room
-    for the longest context)."""
+    for the longest context); beyond it, for all of a step's portions together, every row tile unpacks for itself."""
     key = (lib, nh, nkv, hd, window, first, capacity)
     plans = ctx.__dict__.setdefault("_kv4_plans", {})
     if key in plans:
@@ -1115,8 +1115,9 @@ def paged_attention_kv4(qkv: torch.Tensor, nh: int, nkv: int, hd: int, ctx, cach
                         out: torch.Tensor, first: int = 0) -> None:
     """Causal attention of this step's queries over a 4-bit cache: query head h of the token at position p sees the keys of
     kv head h // (nh / nkv) at positions j <= p with j > p - ``window`` (0: all) or j < ``first``.  ``qkv``: rows that begin
-    with the token's rotated queries, [T, nh * hd] or longer.  Scores, softmax and sums are 32-bit; with bfloat16 rows a
-    probability times its value's scale is rounded to bfloat16."""
+    with the token's rotated queries, [T, nh * hd] or longer.  Scores, softmax and sums are held in 32-bit.  With bfloat16 rows a
+    probability times its value's scale is rounded to bfloat16, and a score's sum over 32 dims carries up to 1,039 times the sum of the
+    row's magnitudes there on its way, so that about 12 * 2^-24 of that may be lost of it."""
     _req(qkv, "qkv", dim=2)
     _req(out, "out", qkv.dtype, 2)
     T, ld = qkv.shape
