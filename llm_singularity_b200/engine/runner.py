@@ -154,6 +154,7 @@ class ModelRunner:
         self._graphs: Dict[tuple, "_StepGraph"] = {}       # (batch size | shape, key of the step's ``after``)
         self._shape_seen: Dict[tuple, int] = {}
         self._shape_order: List[tuple] = []
+        self._portion_captures: Dict[int, bool] = {}       # portion's tokens -> whether capturing it costs no speed
         self.max_shape_graphs = 4
         self.shape_graph_entries = 1
         self.shape_graphs = True
@@ -260,6 +261,8 @@ class ModelRunner:
             return (len(entries), after_key)
         if not self.shape_graphs or len(entries) > self.shape_graph_entries:
             return None
+        if not all(self._captures(len(t)) for t in tokens):
+            return None
         key = (tuple(len(t) for t in tokens), tuple(tuple(e.want) for e in entries), after_key)
         if key in self._graphs:
             self._shape_order.remove(key)
@@ -277,6 +280,14 @@ class ModelRunner:
             self._graphs.pop(self._shape_order.pop(0), None)
         self._shape_order.append(key)
         return key
+
+    def _captures(self, tokens: int) -> bool:
+        """Whether every part runs a portion of ``tokens`` as fast in a captured step as launched for its length."""
+        known = self._portion_captures.get(tokens)
+        if known is None:
+            known = self._portion_captures[tokens] = all(
+                p.captures_portion(tokens, -(-self.max_model_len // self.page_size) * self.page_size) for p in self.model._owners().values())
+        return known
 
     def _step_with_graph(self, key: tuple, entries: Sequence[StepEntry], starts: Sequence[int],
                          moves: List[np.ndarray], source: Optional[torch.Tensor],

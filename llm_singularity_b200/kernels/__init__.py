@@ -1037,6 +1037,26 @@ def _kv4_room(lib: str, hd: int, eights: int, form: int, device) -> int:
     return _kv4_rooms[key]
 
 
+def _kv4_tiles(most: int, seen: int, window: int, first: int) -> int:
+    """Tiles of an expanded cache that a request with up to ``most`` new tokens and ``seen`` in all needs (a window's first tile and the
+    first tokens' last may be cut)."""
+    return -(-(min(seen, window + most + first) if window else seen) // 16) + 2
+
+
+def _kv4_expands(dtype, nkv: int, hd: int, most: int, tiles: int, fixed: bool) -> bool:
+    """Whether portions of up to ``most`` tokens are attended over an expanded cache of ``tiles`` tiles in all."""
+    return dtype == torch.bfloat16 and most >= 128 and hd in _TC_HEAD_DIMS and USE_TCGEN05_ATTENTION \
+        and tiles * nkv * 64 * hd <= (1 << 28 if fixed else 1 << 30)
+
+
+def kv4_portion_captures(dtype, nkv: int, hd: int, tokens: int, table_tokens: int, window: int = 0, first: int = 0) -> bool:
+    """Whether a portion of ``tokens`` is attended as fast in a captured step, which makes room for what block tables of
+    ``table_tokens`` can hold, as in one that knows its length.  (Where it is not, 8B heads and a table of 384,000 tokens, a prompt of
+    32,000 took 1.77 s captured and 0.75 s launched kernel by kernel.)"""
+    return _kv4_expands(dtype, nkv, hd, tokens, _kv4_tiles(tokens, table_tokens, window, first), True) \
+        or not _kv4_expands(dtype, nkv, hd, tokens, _kv4_tiles(tokens, tokens, window, first), False)
+
+
 def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int, capacity: int, device) -> list:
     """The launches of a step's attention over a 4-bit cache, worked out once per step and kind of layer: (mode, offset into the
     per-request arrays, requests, rows of a request, eights of rows of a block, blocks of a cluster, blocks of a spread launch or
@@ -1074,15 +1094,14 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
         evenly = _kv4_room(lib, hd, eights, 1, device)
         # (the longest of the launch's own requests: one long conversation in the step does not make its prompts long)
         seen = capacity if fixed else _portion_keys(ctx) if mode == 2 else int(ctx.h_kv_len.max(where=ctx.h_q_len == 1, initial=0))
+        tiles_seen = _kv4_tiles(most, seen, window, first)
         if window:
             seen = min(seen, window + most + first)
         chunks = -(-seen // 32)                     # the most of a row tile
         splits = spread = parts = 0
-        if mode == 2 and most >= 128 and lib == "attention_kv4" and hd in _TC_HEAD_DIMS and USE_TCGEN05_ATTENTION:
-            tiles_seen = -(-seen // 16) + 2         # (a window's first tile and the first tokens' last may be cut)
-            if count * tiles_seen * nkv * 64 * hd <= (1 << 28 if fixed else 1 << 30):
-                plan.append((3, 4 * at, count, rows, eights, 1, tiles_seen, 0))
-                continue
+        if mode == 2 and _kv4_expands(torch.bfloat16 if lib == "attention_kv4" else torch.float32, nkv, hd, most, count * tiles_seen, fixed):
+            plan.append((3, 4 * at, count, rows, eights, 1, tiles_seen, 0))
+            continue
         cost = None
         for s in range(1, 9):
             rounds = -(-tiles // max(1, _kv4_room(lib, hd, eights, s if s > 1 else 0, device)))

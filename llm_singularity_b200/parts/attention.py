@@ -86,6 +86,11 @@ class PagedAttention(Part):
             return PagedKV4Spec(s.num_kv_heads, s.head_dim, s.window, first)
         return PagedKVSpec(s.num_kv_heads, s.head_dim, s.window, first=first)
 
+    def captures_portion(self, tokens: int, table_tokens: int) -> bool:
+        s, asked = self.spec, getattr(self.rt.ops, "kv4_portion_captures", None)
+        return not self.four_bits or asked is None or asked(self.rt.dtype, s.num_kv_heads, s.head_dim, tokens, table_tokens, s.window or 0,
+                                                            self.first_tokens or 0)
+
     def _modifiers(self) -> dict:
         """Keyword arguments for the attention operations: only what the spec asks for."""
         mods = {}

@@ -330,6 +330,12 @@ class Part:
     """
 
     graph_safe = False
+
+    def captures_portion(self, tokens: int, table_tokens: int) -> bool:
+        """Whether a step that brings a portion of ``tokens`` runs as fast captured, where it is launched for whatever length block
+        tables of ``table_tokens`` can hold, as launched for its own (asked of ``graph_safe`` parts)."""
+        return True
+
     # ``replayable``: everything ``forward`` does on the device goes through the kernel entry points
     # (no tensor-library operations, no values read back), with the same launches for another part
     # of the same spec and the same step, so that a layer's launches can be recorded once and
