@@ -1037,6 +1037,9 @@ def _kv4_room(lib: str, hd: int, eights: int, form: int, device) -> int:
     return _kv4_rooms[key]
 
 
+_kv4_expanded = (1 << 30, 1 << 28)           # bytes that an expanded cache may take, in a step that knows its lengths and in a captured one
+
+
 def _kv4_tiles(most: int, seen: int, window: int, first: int) -> int:
     """Tiles of an expanded cache that a request with up to ``most`` new tokens and ``seen`` in all needs (a window's first tile and the
     first tokens' last may be cut)."""
@@ -1046,7 +1049,7 @@ def _kv4_tiles(most: int, seen: int, window: int, first: int) -> int:
 def _kv4_expands(dtype, nkv: int, hd: int, most: int, tiles: int, fixed: bool) -> bool:
     """Whether portions of up to ``most`` tokens are attended over an expanded cache of ``tiles`` tiles in all."""
     return dtype == torch.bfloat16 and most >= 128 and hd in _TC_HEAD_DIMS and USE_TCGEN05_ATTENTION \
-        and tiles * nkv * 64 * hd <= (1 << 28 if fixed else 1 << 30)
+        and tiles * nkv * 64 * hd <= _kv4_expanded[bool(fixed)]
 
 
 def kv4_portion_captures(dtype, nkv: int, hd: int, tokens: int, table_tokens: int, window: int = 0, first: int = 0) -> bool:
@@ -1077,7 +1080,8 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
     Portions of 128 tokens and more in bfloat16 with heads of 64 or 128 (mode 3) are expanded: what they see is unpacked once, to an
     ordinary cache, for the tcgen05 prompt kernel (2,011 tokens after 4,096, 32 / 8 heads of 128: 1,000 us where every row tile unpacks
     for itself, 229 us so), as long as that cache stays within 1 GB (256 MB in a captured step, which has to have room
-    for the longest context); beyond it, for all of a step's portions together, every row tile unpacks for itself."""
+    for the longest context): all of a step's portions at once, or where they pass it together one after the other.  Beyond it every row
+    tile unpacks for itself."""
     key = (lib, nh, nkv, hd, window, first, capacity)
     plans = ctx.__dict__.setdefault("_kv4_plans", {})
     if key in plans:
@@ -1099,8 +1103,13 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
             seen = min(seen, window + most + first)
         chunks = -(-seen // 32)                     # the most of a row tile
         splits = spread = parts = 0
-        if mode == 2 and _kv4_expands(torch.bfloat16 if lib == "attention_kv4" else torch.float32, nkv, hd, most, count * tiles_seen, fixed):
+        expands = [mode == 2 and _kv4_expands(torch.bfloat16 if lib == "attention_kv4" else torch.float32, nkv, hd, most, n * tiles_seen, fixed)
+                   for n in (count, 1)]
+        if expands[0]:
             plan.append((3, 4 * at, count, rows, eights, 1, tiles_seen, 0))
+            continue
+        if expands[1]:                              # (one after the other where they do not fit together)
+            plan += [(3, 4 * i, 1, int(ctx.h_q_len[i]) * group, eights, 1, tiles_seen, 0) for i in range(at, at + count) if ctx.h_q_len[i] != 1]
             continue
         cost = None
         for s in range(1, 9):

@@ -121,3 +121,13 @@ def test_many_short_requests_are_not_spread(calls, monkeypatch):
     assert _plan(_step([1] * 64, lens(300, 1000)))[1][6] == 0
     assert _plan(_step([1] * 64, lens(1000, 8100)))[1][6] == 444
     assert _plan(_step([1] * 64, [9000] * 64), window=1024, first=4)[1][6] == 0
+
+
+def test_portions_that_pass_the_limit_together_go_one_after_the_other(calls):
+    """Three prompts of 131,072 tokens, single tokens between them: each is unpacked by itself, with the launch arrays of its own place."""
+    ctx = _step([1, 300, 1, 200, 500], [40, 131072, 9, 131072, 100000])
+    plan = ops._kv4_plan(ctx, "attention_kv4", 32, 8, 128, 0, 0, 131072, "cuda:0")
+    assert [p for p in plan if p[0] == 3] == [(3, 4 * i, 1, 4 * n, 2, 1, 8194, 0) for i, n in ((1, 300), (3, 200), (4, 500))]
+    assert [p[0] for p in plan] == [1, 3, 3, 3]
+    assert [p[:3] for p in ops._kv4_plan(_step([300, 200], [100000, 100000]), "attention_kv4", 32, 8, 128, 0, 0, 131072, "cuda:0")] == [(3, 0, 2)]
+    assert [p[0] for p in ops._kv4_plan(_step([300, 200], [300000, 300]), "attention_kv4", 32, 8, 128, 0, 0, 300000, "cuda:0")] == [2]
