@@ -285,8 +285,9 @@ class ModelRunner:
         """Whether every part runs a portion of ``tokens`` as fast in a captured step as launched for its length."""
         known = self._portion_captures.get(tokens)
         if known is None:
-            known = self._portion_captures[tokens] = all(
-                p.captures_portion(tokens, -(-self.max_model_len // self.page_size) * self.page_size) for p in self.model._owners().values())
+            asked = (getattr(p, "captures_portion", None) for p in self.model._owners().values())
+            table = -(-self.max_model_len // self.page_size) * self.page_size
+            known = self._portion_captures[tokens] = all(ask is None or ask(tokens, table) for ask in asked)
         return known
 
     def _step_with_graph(self, key: tuple, entries: Sequence[StepEntry], starts: Sequence[int],

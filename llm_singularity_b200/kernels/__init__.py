@@ -1095,7 +1095,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
         rows = most * group
         eights = 2 if lib == "attention_kv4" and hd <= 128 and rows > 8 else 1
         tiles = requests * nkv * -(-rows // (8 * eights))
-        evenly = _kv4_room(lib, hd, eights, 1, device)
+        evenly = max(1, _kv4_room(lib, hd, eights, 1, device))       # (0: the device takes no such kernel, as the launch will say)
         # (the longest of the launch's own requests: one long conversation in the step does not make its prompts long)
         seen = capacity if fixed else _portion_keys(ctx) if mode == 2 else int(ctx.h_kv_len.max(where=ctx.h_q_len == 1, initial=0))
         tiles_seen = _kv4_tiles(most, seen, window, first)

@@ -131,3 +131,9 @@ def test_portions_that_pass_the_limit_together_go_one_after_the_other(calls):
     assert [p[0] for p in plan] == [1, 3, 3, 3]
     assert [p[:3] for p in ops._kv4_plan(_step([300, 200], [100000, 100000]), "attention_kv4", 32, 8, 128, 0, 0, 131072, "cuda:0")] == [(3, 0, 2)]
     assert [p[0] for p in ops._kv4_plan(_step([300, 200], [300000, 300]), "attention_kv4", 32, 8, 128, 0, 0, 300000, "cuda:0")] == [2]
+
+
+def test_a_device_that_takes_no_such_kernel_is_left_to_say_so(calls, monkeypatch):
+    monkeypatch.setattr(ops, "_kv4_room", lambda *a: 0)
+    for ctx in (_step([1] * 3, [100] * 3), _step([40], [5000]), _step([1], [5], fixed=True)):
+        assert len(ops._kv4_plan(ctx, "attention_kv4_f32", 8, 2, 64, 0, 0, 8192, "cuda:0")) == 1
