@@ -1079,7 +1079,7 @@ def _kv4_plan(ctx, lib: str, nh: int, nkv: int, hd: int, window: int, first: int
 
     Portions of 128 tokens and more in bfloat16 with heads of 64 or 128 (mode 3) are expanded: what they see is unpacked once, to an
     ordinary cache, for the tcgen05 prompt kernel (2,011 tokens after 4,096, 32 / 8 heads of 128: 1,000 us where every row tile unpacks
-    for itself, 229 us so), as long as that cache stays within 1 GB (256 MB in a captured step, which has to have room
+    for itself, 231 us so), as long as that cache stays within 1 GB (256 MB in a captured step, which has to have room
     for the longest context): all of a step's portions at once, or where they pass it together one after the other.  Beyond it every row
     tile unpacks for itself."""
     key = (lib, nh, nkv, hd, window, first, capacity)
